@@ -606,6 +606,88 @@ int cgn_gemm_bb_wants(int32_t M, int32_t N, int32_t K);
 int cgn_cast_bf16_f32(void* stream, const float* src, cgn_axis rows, int32_t n_rows, int32_t n_cols, void* dst,
                       int64_t ld_dst, int32_t transpose);
 
+/* ------------------------------------------------------------------------------------------------------------
+ * Operators for tuning the generator on its own samples. Rows of `bf16` != 0 tensors hold bfloat16 (strides in elements),
+ * else float; parameters, statistics and losses are float.
+ * ---------------------------------------------------------------------------------------------------------- */
+/* Layer norm over the last axis of x [R, C] (row stride ldx, 1 <= C <= 8192; csrc/layernorm.hip):
+ *   mean[r], rstd[r] = 1 / sqrt(var + eps);  y = (x - mean) * rstd * weight + bias   (weight / bias null: 1 / 0).
+ * y may be x's own buffer. */
+int cgn_layer_norm_fwd(void* stream, const void* x, int64_t ldx, int64_t R, int32_t C, int32_t bf16, const float* weight,
+                       const float* bias, float eps, void* y, int64_t ldy, float* mean, float* rstd);
+/* Its backward pass, from the statistics of the forward pass: dx (nullable; may be dy's or x's own buffer) and
+ * dweight / dbias = beta * itself + the sums over the rows (nullable; R == 0 gives sums of zero).
+ * workspace (with dweight or dbias): min(R, 512) * 2 * C * 4 bytes. */
+int cgn_layer_norm_bwd(void* stream, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t R, int32_t C,
+                       int32_t bf16, const float* weight, const float* mean, const float* rstd, void* dx, int64_t lddx,
+                       float* dweight, float* dbias, float beta, float* workspace, int64_t workspace_bytes);
+
+/* Sampled tokens: row i of logits [M, V] (row stride ld) gave token target[i]. Rows with weight[i] == 0 are neither read
+ * nor scored (log-probability and gradient zero, whatever they hold); weight null: 1 everywhere. A target outside
+ * [0, V) in a row that counts gives NaN. inv_tau > 0 (dyn_inv_tau: nullable device override). */
+typedef struct cgn_token_rows {
+    const void* logits;
+    int64_t ld;
+    int64_t M;
+    const int64_t* target;
+    const float* weight;
+    const float* dyn_inv_tau;
+    int32_t V;
+    int32_t bf16;
+    float inv_tau;
+} cgn_token_rows;
+
+/* logp[i] = log softmax(inv_tau * logits[i])[target[i]]; stats [M][2] (nullable) = the row's maximum and sum, which the
+ * gradient takes (csrc/token_loss.hip). */
+int cgn_token_logp(void* stream, const cgn_token_rows* rows, float* logp, float* stats);
+/* dlogits[i] = scale[0] * coef[i] * d logp[i] / d logits[i] (scale null: 1; zeros in rows of weight 0). coef holds the
+ * whole factor of a row, its weight included. dlogits may be the logits' own buffer. */
+int cgn_token_logp_bwd(void* stream, const cgn_token_rows* rows, const float* stats, const float* coef,
+                       const float* scale, void* dlogits, int64_t ldd);
+/* Clipped policy loss with a KL term, over log-probabilities lp of the sampled tokens:
+ *   rho = exp(lp - old_logp) (old_logp null: 1),  k = ref_logp - lp
+ *   loss = sum_i weight_i * (-min(rho A, clip(rho, 1 - clip_lo, 1 + clip_hi) A) + kl_coef * (exp(k) - k - 1))
+ * with A = advantage; ref_logp null: no KL term. logp [M]; stats [M][2] and coef [M] (both nullable) are what
+ * cgn_token_logp_bwd takes; dlogits (nullable; may be the logits' own buffer) gets the gradient of the loss.
+ * workspace: 24 * M + 16 bytes, 8-byte aligned. */
+int cgn_policy_loss(void* stream, const cgn_token_rows* rows, const float* advantage, const float* old_logp,
+                    const float* ref_logp, float clip_lo, float clip_hi, float kl_coef, float* loss, float* logp,
+                    float* stats, float* coef, void* dlogits, int64_t ldd, void* workspace, int64_t workspace_bytes);
+/* Preference loss over P = M / (2 T) pairs of sentences of T rows each (sentences 0..P-1 chosen, P..2P-1 rejected):
+ *   S_j = sum_t weight * lp,  m_p = beta * ((S_p - ref_p) - (S_{P+p} - ref_{P+p}))
+ *   loss = mean_p (-(1 - label_smoothing) log sigmoid(m_p) - label_smoothing log sigmoid(-m_p))
+ * beta > 0, 0 <= label_smoothing < 0.5; margin [P] = m, seq_logp [2P] = S; stats, coef, dlogits and workspace as above. */
+int cgn_preference_loss(void* stream, const cgn_token_rows* rows, int32_t T, const float* ref_logp, double beta,
+                        double label_smoothing, float* loss, float* margin, float* seq_logp, float* stats, float* coef,
+                        void* dlogits, int64_t ldd, void* workspace, int64_t workspace_bytes);
+
+/* One gradient tensor of a list (host memory): rows x cols elements; rows == 1: cols elements in one piece, else a matrix
+ * with row strides ld (g) and ldo (out). bf16 as above. */
+typedef struct cgn_grad_tensor {
+    const void* g;
+    void* out;
+    int64_t rows;
+    int64_t cols;
+    int64_t ld;
+    int64_t ldo;
+    int64_t bf16;
+} cgn_grad_tensor;
+
+/* Bytes of workspace that the two calls below need for this list (host call; 8-byte aligned). */
+int cgn_grad_norm_workspace(const cgn_grad_tensor* t, int32_t n, int64_t* bytes);
+/* norm[0] = |scale| * sqrt(sum g^2) over all tensors (max_abs != 0: |scale| * max |g|); coef (nullable)
+ * [0] = min(1, max_norm / (norm + 1e-6)). NaN gradients give NaN (csrc/gradnorm.hip). */
+int cgn_grad_norm(void* stream, const cgn_grad_tensor* t, int32_t n, int32_t max_abs, double scale, double max_norm,
+                  float* norm, float* coef, void* workspace, int64_t workspace_bytes);
+/* The same norm, and out = g * scale * min(1, max_norm / (norm + 1e-6)) for every tensor (out may be g). Tensors must not
+ * overlap each other. */
+int cgn_clip_grads(void* stream, const cgn_grad_tensor* t, int32_t n, int32_t max_abs, double scale, double max_norm,
+                   float* norm, void* workspace, int64_t workspace_bytes);
+/* cgn_adam_f32 with the gradients read as g * grad_scale * clip_coef[0] (device): the update behind cgn_grad_norm. */
+int cgn_adam_clipped_f32(void* stream, float* p, const float* g, float* m, float* v, int64_t n, float lr, float beta1,
+                         float beta2, float eps, int32_t step, const int32_t* dyn_step, float grad_scale,
+                         const float* clip_coef);
+
 #ifdef __cplusplus
 }
 #endif

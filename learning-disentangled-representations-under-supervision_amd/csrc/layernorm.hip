@@ -1,0 +1,359 @@
+// Layer norm over the last axis of [R, C] rows, forward and backward (hip/ops.py layer_norm_fwd / layer_norm_bwd).
+//   mu = mean(x), var = mean((x - mu)^2), r = 1 / sqrt(var + eps), xh = (x - mu) r, y = xh w + b
+//   g = dy w,  dx = r (g - mean(g) - xh mean(g xh)),  dw = sum over rows dy xh,  db = sum over rows dy
+// HBM-bound (8 to 22 flops per element): every row is read once into registers and stays there for all its sums. A group
+// of G lanes owns a row; each lane holds NV 16-byte pieces of it.
+#include "rows.h"
+
+namespace {
+
+using namespace cgn_rows;
+
+// Sums over the row's group: inside the wave with shuffles, over a whole workgroup through LDS.
+template <int NT, int G, int K>
+__device__ __forceinline__ void row_sums(float (&s)[K], float* red) {
+    static_assert(G <= 64 || G == NT, "a group is part of a wave or the whole workgroup");
+#pragma unroll
+    for (int k = 0; k < K; ++k) s[k] = group_sum<(G < 64 ? G : 64)>(s[k]);
+    if constexpr (G > 64) {
+        __syncthreads();  // (the previous call's readers are done)
+        if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) red[(threadIdx.x >> 6) * K + k] = s[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            s[k] = 0.f;
+#pragma unroll
+            for (int w = 0; w < G / 64; ++w) s[k] += red[w * K + k];
+        }
+    }
+}
+
+// A row as its group holds it: lane l has the pieces l, l + G, ... of the C / E whole ones, and lane l < C % E the single
+// element behind them. What a lane does not have reads as zero.
+template <typename T, int NV, int G>
+struct Row {
+    Piece<T> q[NV];
+    float t;
+    __device__ __forceinline__ void load(const T* row, int lane, int nfull, int rem) {
+        constexpr int E = Piece<T>::E;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int i = lane + j * G;
+            if (i < nfull)
+                q[j].load(row + (long)i * E);
+            else
+                q[j].fill(0.f);
+        }
+        t = lane < rem ? Piece<T>::one(row + nfull * E + lane) : 0.f;
+    }
+};
+
+// The group's share of a parameter vector (null: `none` everywhere), laid out like a Row.
+template <int NV, int E, int G>
+struct Param {
+    float v[NV][E], t;
+    __device__ __forceinline__ void load(const float* w, float none, int lane, int nfull, int rem) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int i = lane + j * G;
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[j][e] = none;
+            if (w && i < nfull) {
+#pragma unroll
+                for (int h = 0; h < E / 4; ++h) {
+                    Piece<float> p;
+                    p.load(w + (long)i * E + 4 * h);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[j][4 * h + e] = p.get(e);
+                }
+            }
+        }
+        t = w && lane < rem ? w[nfull * E + lane] : none;
+    }
+};
+
+// One row per group. Two sums are taken: the mean, then (both at once) the sums of d = x - mean and d^2; the first of them
+// is what the mean's own rounding left over, so rows whose mean is large against their spread keep fp32 accuracy.
+template <typename T, int NT, int G, int NV>
+__global__ __launch_bounds__(NT) void layer_norm_fwd_kernel(const T* x, long ldx, long R, int C,
+                                                            const float* __restrict__ w, const float* __restrict__ b,
+                                                            float eps, T* y, long ldy, float* __restrict__ mean,
+                                                            float* __restrict__ rstd) {
+    constexpr int E = Piece<T>::E;
+    __shared__ float red[NT / 64 * 2];
+    const int lane = threadIdx.x % G;
+    const int nfull = C / E, rem = C % E;
+    const float inv_c = 1.f / (float)C;
+    Param<NV, E, G> pw, pb;
+    pw.load(w, 1.f, lane, nfull, rem);
+    pb.load(b, 0.f, lane, nfull, rem);
+    for (long r = (long)blockIdx.x * (NT / G) + threadIdx.x / G; r < R; r += (long)gridDim.x * (NT / G)) {
+        Row<T, NV, G> row;
+        row.load(x + r * ldx, lane, nfull, rem);
+        float s1[1] = {row.t};
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int e = 0; e < E; ++e) s1[0] += row.q[j].get(e);
+        row_sums<NT, G, 1>(s1, red);
+        const float mu = s1[0] * inv_c;
+        float s2[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (lane + j * G < nfull) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float d = row.q[j].get(e) - mu;
+                    s2[0] += d;
+                    s2[1] += d * d;
+                }
+            }
+        if (lane < rem) {
+            const float d = row.t - mu;
+            s2[0] += d;
+            s2[1] += d * d;
+        }
+        row_sums<NT, G, 2>(s2, red);
+        const float off = s2[0] * inv_c;
+        const float v = s2[1] * inv_c - off * off;
+        const float rs = 1.f / sqrtf((v < 0.f ? 0.f : v) + eps);  // (a NaN stays one)
+        if (lane == 0) {
+            mean[r] = mu + off;
+            rstd[r] = rs;
+        }
+        T* yr = y + r * ldy;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int i = lane + j * G;
+            if (i < nfull) {
+                float o[E];
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] = ((row.q[j].get(e) - mu) - off) * rs * pw.v[j][e] + pb.v[j][e];
+                Piece<T>::store(yr + (long)i * E, o);
+            }
+        }
+        if (lane < rem) Piece<T>::put(yr + nfull * E + lane, ((row.t - mu) - off) * rs * pw.t + pb.t);
+    }
+}
+
+// Backward. Every group walks rows r, r + step, ...; its columns' shares of dw and db stay in registers and leave the
+// workgroup once, as one [2][C] row of `part` per workgroup (fixed order: no atomics, the same bits every run).
+// dx may be dy's or x's own buffer: a row is in registers before anything of it is written.
+template <typename T, int NT, int G, int NV>
+__global__ __launch_bounds__(NT) void layer_norm_bwd_kernel(const T* dy, long lddy, const T* x, long ldx, long R, int C,
+                                                            const float* __restrict__ w, const float* __restrict__ mean,
+                                                            const float* __restrict__ rstd, T* dx, long lddx,
+                                                            float* __restrict__ part) {
+    constexpr int E = Piece<T>::E;
+    constexpr int GROUPS = NT / G;
+    __shared__ float red[NT / 64 * 3];
+    const int lane = threadIdx.x % G, grp = threadIdx.x / G;
+    const int nfull = C / E, rem = C % E;
+    const float inv_c = 1.f / (float)C;
+    Param<NV, E, G> pw;
+    pw.load(w, 1.f, lane, nfull, rem);
+    float aw[NV][E], ab[NV][E], awt = 0.f, abt = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < E; ++e) aw[j][e] = ab[j][e] = 0.f;
+    for (long r = (long)blockIdx.x * GROUPS + grp; r < R; r += (long)gridDim.x * GROUPS) {
+        Row<T, NV, G> qx, qd;
+        qx.load(x + r * ldx, lane, nfull, rem);
+        qd.load(dy + r * lddy, lane, nfull, rem);
+        const float mu = mean[r], rs = rstd[r];
+        // sums of xh, g and g xh: the first is what the stored mean's rounding left in xh, taken out below
+        float s[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (lane + j * G < nfull) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float xh = (qx.q[j].get(e) - mu) * rs, g = qd.q[j].get(e) * pw.v[j][e];
+                    s[0] += xh;
+                    s[1] += g;
+                    s[2] += g * xh;
+                }
+            }
+        const float xht = lane < rem ? (qx.t - mu) * rs : 0.f, gt = qd.t * pw.t;
+        s[0] += xht;
+        s[1] += gt;
+        s[2] += gt * xht;
+        row_sums<NT, G, 3>(s, red);
+        const float off = s[0] * inv_c, mg = s[1] * inv_c, mgx = s[2] * inv_c - mg * off;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int i = lane + j * G;
+            if (i < nfull) {
+                float o[E];
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float d = qd.q[j].get(e);
+                    const float xh = (qx.q[j].get(e) - mu) * rs - off;
+                    aw[j][e] += d * xh;
+                    ab[j][e] += d;
+                    o[e] = rs * ((d * pw.v[j][e] - mg) - xh * mgx);
+                }
+                if (dx) Piece<T>::store(dx + r * lddx + (long)i * E, o);
+            }
+        }
+        if (lane < rem) {
+            awt += qd.t * (xht - off);
+            abt += qd.t;
+            if (dx) Piece<T>::put(dx + r * lddx + nfull * E + lane, rs * ((gt - mg) - (xht - off) * mgx));
+        }
+    }
+    if (!part) return;
+    // the workgroup's groups summed in a fixed order, one piece of every lane at a time through LDS
+    float* out = part + (long)blockIdx.x * 2 * C;
+    __shared__ float rows[GROUPS][GROUPS > 1 ? G * E : 1];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int j = 0; j <= NV; ++j) {
+            const int width = j < NV ? E : 1;            // (the last round: the single elements)
+            const int col0 = j < NV ? j * G * E : nfull * E;
+            const int cend = j < NV ? nfull * E : C;
+            if constexpr (GROUPS == 1) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    if (e >= width) break;
+                    const int c = col0 + lane * width + e;
+                    const float v = j < NV ? (k ? ab[j < NV ? j : 0][e] : aw[j < NV ? j : 0][e]) : (k ? abt : awt);
+                    if (c < cend) out[k * C + c] = v;
+                }
+            } else {
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    if (e >= width) break;
+                    rows[grp][lane * width + e] =
+                        j < NV ? (k ? ab[j < NV ? j : 0][e] : aw[j < NV ? j : 0][e]) : (k ? abt : awt);
+                }
+                __syncthreads();
+                for (int c = threadIdx.x; c < G * width; c += NT) {
+                    float t = 0.f;
+#pragma unroll
+                    for (int q = 0; q < GROUPS; ++q) t += rows[q][c];
+                    if (col0 + c < cend) out[k * C + col0 + c] = t;
+                }
+            }
+        }
+    }
+}
+
+// dw[c] = beta dw[c] + sum over the workgroups' rows of part, in a fixed order; db likewise.
+constexpr int LNF_NT = 1024;
+__global__ __launch_bounds__(LNF_NT) void layer_norm_params_kernel(const float* __restrict__ part, int nb, int C,
+                                                                   float beta, float* __restrict__ dw,
+                                                                   float* __restrict__ db) {
+    __shared__ float red[LNF_NT / 64][64];
+    const int lane = threadIdx.x & 63, seg = threadIdx.x >> 6;
+    const int c = blockIdx.x * 64 + lane;
+    float t = 0.f;
+    if (c < 2 * C) {
+#pragma unroll 8
+        for (int i = seg; i < nb; i += LNF_NT / 64) t += part[(long)i * 2 * C + c];
+    }
+    red[seg][lane] = t;
+    __syncthreads();
+    if (seg == 0 && c < 2 * C) {
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < LNF_NT / 64; ++k) v += red[k][lane];
+        float* o = c < C ? dw : db;
+        if (!o) return;
+        o += c < C ? c : c - C;
+        *o = beta != 0.f ? v + beta * *o : v;
+    }
+}
+
+constexpr int LN_MAX_C = 8192;    // widest row that LN_DISPATCH's groups hold in registers
+constexpr int LN_FWD_NB = 2048;   // workgroups of a forward pass at most: what is resident at once, each with many rows
+constexpr int LN_BWD_NB = 512;    // workgroups of a backward pass at most: rows of `part` it reduces at the end
+
+template <typename T, int NT, int G, int NV>
+int launch_fwd(hipStream_t s, const void* x, int64_t ldx, int64_t R, int C, const float* w, const float* b, float eps,
+               void* y, int64_t ldy, float* mean, float* rstd) {
+    int64_t nb = (R + NT / G - 1) / (NT / G);
+    if (nb > LN_FWD_NB) nb = LN_FWD_NB;
+    hipLaunchKernelGGL((layer_norm_fwd_kernel<T, NT, G, NV>), dim3((unsigned)nb), dim3(NT), 0, s, (const T*)x, (long)ldx,
+                       (long)R, C, w, b, eps, (T*)y, (long)ldy, mean, rstd);
+    CGN_LAUNCH_CHECK();
+    return CGN_OK;
+}
+
+template <typename T, int NT, int G, int NV>
+int launch_bwd(hipStream_t s, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t R, int C, const float* w,
+               const float* mean, const float* rstd, void* dx, int64_t lddx, float* dw, float* db, float beta,
+               float* part, int64_t part_bytes) {
+    int64_t nb = (R + NT / G - 1) / (NT / G);
+    if (nb > LN_BWD_NB) nb = LN_BWD_NB;
+    const bool params = dw || db;
+    if (params && nb * 2 * C * 4 > part_bytes) return CGN_ERR_WORKSPACE;
+    if (nb > 0) {
+        hipLaunchKernelGGL((layer_norm_bwd_kernel<T, NT, G, NV>), dim3((unsigned)nb), dim3(NT), 0, s, (const T*)dy,
+                           (long)lddy, (const T*)x, (long)ldx, (long)R, C, w, mean, rstd, (T*)dx, (long)lddx,
+                           params ? part : nullptr);
+        CGN_LAUNCH_CHECK();
+    }
+    if (params) {
+        hipLaunchKernelGGL(layer_norm_params_kernel, dim3(cgn_cdiv(2L * C, 64)), dim3(LNF_NT), 0, s, part, (int)nb, C, beta,
+                           dw, db);
+        CGN_LAUNCH_CHECK();
+    }
+    return CGN_OK;
+}
+
+// The narrowest group whose lanes hold the row in at most 16 elements each (with the backward pass's sums that is what
+// stays in registers): narrow rows share a wave, wide ones take a workgroup.
+#define LN_DISPATCH(fn, ...)                                                      \
+    do {                                                                          \
+        const int n__ = cgn_cdiv(C, bf16 ? 8 : 4); /* pieces of a row */          \
+        if (bf16) {                                                               \
+            if (n__ <= 8) return fn<Bf16, 256, 8, 1>(__VA_ARGS__);                \
+            if (n__ <= 16) return fn<Bf16, 256, 16, 1>(__VA_ARGS__);              \
+            if (n__ <= 32) return fn<Bf16, 256, 32, 1>(__VA_ARGS__);              \
+            if (n__ <= 64) return fn<Bf16, 256, 64, 1>(__VA_ARGS__);              \
+            if (n__ <= 128) return fn<Bf16, 256, 64, 2>(__VA_ARGS__);             \
+            if (n__ <= 256) return fn<Bf16, 256, 256, 1>(__VA_ARGS__);            \
+            if (n__ <= 512) return fn<Bf16, 256, 256, 2>(__VA_ARGS__);            \
+            return fn<Bf16, 1024, 1024, 1>(__VA_ARGS__);                          \
+        }                                                                         \
+        if (n__ <= 8) return fn<float, 256, 8, 1>(__VA_ARGS__);                   \
+        if (n__ <= 16) return fn<float, 256, 16, 1>(__VA_ARGS__);                 \
+        if (n__ <= 32) return fn<float, 256, 32, 1>(__VA_ARGS__);                 \
+        if (n__ <= 64) return fn<float, 256, 64, 1>(__VA_ARGS__);                 \
+        if (n__ <= 128) return fn<float, 256, 64, 2>(__VA_ARGS__);                \
+        if (n__ <= 256) return fn<float, 256, 64, 4>(__VA_ARGS__);                \
+        if (n__ <= 512) return fn<float, 256, 256, 2>(__VA_ARGS__);               \
+        if (n__ <= 1024) return fn<float, 256, 256, 4>(__VA_ARGS__);              \
+        return fn<float, 1024, 1024, 2>(__VA_ARGS__);                             \
+    } while (0)
+
+}  // namespace
+
+extern "C" int cgn_layer_norm_fwd(void* stream, const void* x, int64_t ldx, int64_t R, int32_t C, int32_t bf16,
+                                  const float* weight, const float* bias, float eps, void* y, int64_t ldy, float* mean,
+                                  float* rstd) {
+    CGN_CHECK_ARG(R >= 0 && C > 0 && C <= LN_MAX_C && ldx >= C && ldy >= C && eps >= 0.f);
+    if (R == 0) return CGN_OK;
+    CGN_CHECK_ARG(x && y && mean && rstd);
+    hipStream_t s = (hipStream_t)stream;
+    LN_DISPATCH(launch_fwd, s, x, ldx, R, C, weight, bias, eps, y, ldy, mean, rstd);
+}
+
+extern "C" int cgn_layer_norm_bwd(void* stream, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t R,
+                                  int32_t C, int32_t bf16, const float* weight, const float* mean, const float* rstd,
+                                  void* dx, int64_t lddx, float* dweight, float* dbias, float beta, float* workspace,
+                                  int64_t workspace_bytes) {
+    CGN_CHECK_ARG(R >= 0 && C > 0 && C <= LN_MAX_C && lddy >= C && ldx >= C && (!dx || lddx >= C));
+    CGN_CHECK_ARG(R == 0 || (dy && x && mean && rstd));
+    CGN_CHECK_ARG((!dweight && !dbias) || R == 0 || workspace);
+    hipStream_t s = (hipStream_t)stream;
+    LN_DISPATCH(launch_bwd, s, dy, lddy, x, ldx, R, C, weight, mean, rstd, dx, lddx, dweight, dbias, beta, workspace,
+                workspace_bytes);
+}

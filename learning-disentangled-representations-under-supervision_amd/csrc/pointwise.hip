@@ -234,7 +234,9 @@ __global__ __launch_bounds__(PW_NT) void rowdot_kernel(const float* __restrict__
 __global__ __launch_bounds__(PW_NT) void adam_kernel(float* __restrict__ p, const float* __restrict__ g,
                                                      float* __restrict__ m, float* __restrict__ v, long n, float lr,
                                                      float b1, float b2, float eps, float bc1, float bc2_sqrt,
-                                                     const int* __restrict__ dyn_step, float grad_scale) {
+                                                     const int* __restrict__ dyn_step, float grad_scale,
+                                                     const float* __restrict__ clip_coef) {
+    if (clip_coef) grad_scale *= clip_coef[0];
     if (dyn_step) {  // device-resident step count: same double-precision bias corrections as the host path
         const double t = (double)dyn_step[0];
         bc1 = (float)(1.0 - pow((double)b1, t));
@@ -258,7 +260,9 @@ __global__ __launch_bounds__(PW_NT) void adam_kernel(float* __restrict__ p, cons
 __global__ __launch_bounds__(PW_NT) void adam_vec4_kernel(float* __restrict__ p, const float* __restrict__ g,
                                                           float* __restrict__ m, float* __restrict__ v, long n, float lr,
                                                           float b1, float b2, float eps, float bc1, float bc2_sqrt,
-                                                          const int* __restrict__ dyn_step, float grad_scale) {
+                                                          const int* __restrict__ dyn_step, float grad_scale,
+                                                          const float* __restrict__ clip_coef) {
+    if (clip_coef) grad_scale *= clip_coef[0];
     if (dyn_step) {
         const double t = (double)dyn_step[0];
         bc1 = (float)(1.0 - pow((double)b1, t));
@@ -648,8 +652,8 @@ extern "C" int cgn_rowdot_f32(void* stream, const float* a, int64_t lda, const f
     return CGN_OK;
 }
 
-extern "C" int cgn_adam_f32(void* stream, float* p, const float* g, float* m, float* v, int64_t n, float lr, float beta1,
-                            float beta2, float eps, int32_t step, const int32_t* dyn_step, float grad_scale) {
+static int adam(void* stream, float* p, const float* g, float* m, float* v, int64_t n, float lr, float beta1, float beta2,
+                float eps, int32_t step, const int32_t* dyn_step, float grad_scale, const float* clip_coef) {
     CGN_CHECK_ARG(n >= 0 && (dyn_step || step >= 1));
     if (n == 0) return CGN_OK;
     CGN_CHECK_ARG(p && g && m && v);
@@ -660,12 +664,24 @@ extern "C" int cgn_adam_f32(void* stream, float* p, const float* g, float* m, fl
     const bool vec = (((uintptr_t)p | (uintptr_t)g | (uintptr_t)m | (uintptr_t)v) % 16 == 0) && n >= 4;
     if (vec)
         hipLaunchKernelGGL(adam_vec4_kernel, dim3(pw_blocks(n / 4, PW_NT, 8192)), dim3(PW_NT), 0, S_(stream), p, g, m, v,
-                           (long)n, lr, beta1, beta2, eps, (float)bc1, (float)sqrt(bc2), dyn_step, grad_scale);
+                           (long)n, lr, beta1, beta2, eps, (float)bc1, (float)sqrt(bc2), dyn_step, grad_scale, clip_coef);
     else
         hipLaunchKernelGGL(adam_kernel, dim3(pw_blocks(n, PW_NT, 8192)), dim3(PW_NT), 0, S_(stream), p, g, m, v, (long)n,
-                           lr, beta1, beta2, eps, (float)bc1, (float)sqrt(bc2), dyn_step, grad_scale);
+                           lr, beta1, beta2, eps, (float)bc1, (float)sqrt(bc2), dyn_step, grad_scale, clip_coef);
     CGN_LAUNCH_CHECK();
     return CGN_OK;
+}
+
+extern "C" int cgn_adam_f32(void* stream, float* p, const float* g, float* m, float* v, int64_t n, float lr, float beta1,
+                            float beta2, float eps, int32_t step, const int32_t* dyn_step, float grad_scale) {
+    return adam(stream, p, g, m, v, n, lr, beta1, beta2, eps, step, dyn_step, grad_scale, nullptr);
+}
+
+extern "C" int cgn_adam_clipped_f32(void* stream, float* p, const float* g, float* m, float* v, int64_t n, float lr,
+                                    float beta1, float beta2, float eps, int32_t step, const int32_t* dyn_step,
+                                    float grad_scale, const float* clip_coef) {
+    CGN_CHECK_ARG(clip_coef);
+    return adam(stream, p, g, m, v, n, lr, beta1, beta2, eps, step, dyn_step, grad_scale, clip_coef);
 }
 
 extern "C" int cgn_incr_i32(void* stream, int32_t* counter) {

@@ -28,6 +28,7 @@ c_float_p = C.c_void_p  # raw device pointers travel as integers
 c_i64 = C.c_int64
 c_i32 = C.c_int32
 c_f32 = C.c_float
+c_f64 = C.c_double
 c_ptr = C.c_void_p
 
 
@@ -111,6 +112,16 @@ class ConvWidths(C.Structure):
                 ("n", c_i32), ("F", c_i32), ("act", c_i32), ("layout", c_i32)]
 
 
+class TokenRows(C.Structure):
+    _fields_ = [("logits", c_ptr), ("ld", c_i64), ("M", c_i64), ("target", c_ptr), ("weight", c_ptr),
+                ("dyn_inv_tau", c_ptr), ("V", c_i32), ("bf16", c_i32), ("inv_tau", c_f32)]
+
+
+class GradTensor(C.Structure):
+    _fields_ = [("g", c_ptr), ("out", c_ptr), ("rows", c_i64), ("cols", c_i64), ("ld", c_i64), ("ldo", c_i64),
+                ("bf16", c_i64)]
+
+
 ACT_RELU = 0
 ACT_TANH = 1
 
@@ -185,6 +196,21 @@ PROTOTYPES = {
     "cgn_lincomb_f32": (c_i32, [c_ptr, c_i32, C.POINTER(c_ptr), C.POINTER(c_f32), c_ptr]),
     "cgn_gemm_bb": (c_i32, [c_ptr, C.POINTER(GemmBBDesc), c_ptr, c_ptr, C.POINTER(c_i32), C.POINTER(c_i32)]),
     "cgn_gemm_bb_wants": (c_i32, [c_i32, c_i32, c_i32]),
+    "cgn_layer_norm_fwd": (c_i32, [c_ptr, c_ptr, c_i64, c_i64, c_i32, c_i32, c_ptr, c_ptr, c_f32, c_ptr, c_i64, c_ptr,
+                                   c_ptr]),
+    "cgn_layer_norm_bwd": (c_i32, [c_ptr, c_ptr, c_i64, c_ptr, c_i64, c_i64, c_i32, c_i32, c_ptr, c_ptr, c_ptr, c_ptr,
+                                   c_i64, c_ptr, c_ptr, c_f32, c_ptr, c_i64]),
+    "cgn_token_logp": (c_i32, [c_ptr, C.POINTER(TokenRows), c_ptr, c_ptr]),
+    "cgn_token_logp_bwd": (c_i32, [c_ptr, C.POINTER(TokenRows), c_ptr, c_ptr, c_ptr, c_ptr, c_i64]),
+    "cgn_policy_loss": (c_i32, [c_ptr, C.POINTER(TokenRows), c_ptr, c_ptr, c_ptr, c_f32, c_f32, c_f32, c_ptr, c_ptr, c_ptr,
+                                c_ptr, c_ptr, c_i64, c_ptr, c_i64]),
+    "cgn_preference_loss": (c_i32, [c_ptr, C.POINTER(TokenRows), c_i32, c_ptr, c_f64, c_f64, c_ptr, c_ptr, c_ptr, c_ptr,
+                                    c_ptr, c_ptr, c_i64, c_ptr, c_i64]),
+    "cgn_grad_norm_workspace": (c_i32, [c_ptr, c_i32, C.POINTER(c_i64)]),
+    "cgn_grad_norm": (c_i32, [c_ptr, c_ptr, c_i32, c_i32, c_f64, c_f64, c_ptr, c_ptr, c_ptr, c_i64]),
+    "cgn_clip_grads": (c_i32, [c_ptr, c_ptr, c_i32, c_i32, c_f64, c_f64, c_ptr, c_ptr, c_i64]),
+    "cgn_adam_clipped_f32": (c_i32, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_f32, c_f32, c_f32, c_f32, c_i32, c_ptr,
+                                     c_f32, c_ptr]),
     "cgn_cast_bf16_f32": (c_i32, [c_ptr, c_ptr, Axis, c_i32, c_i32, c_ptr, c_i64, c_i32]),
 }
 

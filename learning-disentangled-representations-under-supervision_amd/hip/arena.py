@@ -125,18 +125,22 @@ class AdamState:
         # bumps it with cgn_incr_i32 and the Adam kernel forms the bias corrections from it)
         self.step_dev = torch.zeros(1, dtype=torch.int32, device=arena.p.device)
 
-    def apply(self, lr, grad_scale=1.0, betas=(0.9, 0.999), eps=1e-8, dynamic=False):
+    def apply(self, lr, grad_scale=1.0, betas=(0.9, 0.999), eps=1e-8, dynamic=False, max_norm=None):
         """One Adam update. dynamic=True reads (and first increments) the device step count instead of the host's;
-        the caller (hip/graph.py) keeps `self.step` in line with it."""
+        the caller (hip/graph.py) keeps `self.step` in line with it. max_norm: clip this group's gradient to that 2-norm
+        (the arena's padding is zero and adds nothing); returns the norm before clipping, a device tensor, else None."""
         a = self.arena
         if dynamic:
             ops.incr(self.step_dev)
             if a.size:
-                ops.adam(a.p, a.g, self.m, self.v, lr, 0, betas[0], betas[1], eps, grad_scale, dyn_step=self.step_dev)
-            return
+                return ops.adam(a.p, a.g, self.m, self.v, lr, 0, betas[0], betas[1], eps, grad_scale,
+                                dyn_step=self.step_dev, max_norm=max_norm)
+            return None
         self.step += 1
         if a.size:
-            ops.adam(a.p, a.g, self.m, self.v, lr, self.step, betas[0], betas[1], eps, grad_scale)
+            return ops.adam(a.p, a.g, self.m, self.v, lr, self.step, betas[0], betas[1], eps, grad_scale,
+                            max_norm=max_norm)
+        return None
 
     def sync_device_step(self):
         self.step_dev.fill_(self.step)

@@ -319,3 +319,116 @@ def embedding_lookup(idx, table):
     out = new((flat.numel(), table.shape[1]), table.device)
     ops.gather_rows(table.detach(), flat, out)
     return out.view(*idx.shape, table.shape[1])
+
+
+# ------------------------------------------------------------------------------------------------------------------
+def _packed(t):
+    """Contiguous float32 / bfloat16 tensor (autograd may hand over an expanded or strided gradient)."""
+    return t if t.is_contiguous() else t.contiguous()
+
+
+class _LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, W, b, eps):
+        need_cuda(x, "LayerNorm")
+        x = _packed(x)
+        y, mean, rstd = ops.layer_norm_fwd(x, W, b, eps)
+        ctx.save_for_backward(x, W, mean, rstd)
+        ctx.has_bias = b is not None
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, W, mean, rstd = ctx.saved_tensors
+        need_dx, need_dw, need_db = ctx.needs_input_grad[:3]
+        dx, dW, db = ops.layer_norm_bwd(_packed(dy), x, W, mean, rstd, dx=None if need_dx else False,
+                                        params=need_dw or need_db)
+        return dx if need_dx else None, dW if need_dw else None, db if need_db else None, None
+
+
+class LayerNorm(nn.Module):
+    """nn.LayerNorm over the last axis (same parameter names / default init): float32 or bfloat16 activations with any
+    leading axes, float32 parameters."""
+
+    def __init__(self, features, eps=1e-5, elementwise_affine=True, bias=True):
+        super().__init__()
+        if not 1 <= features <= ops.LAYER_NORM_MAX_COLS:
+            raise ValueError("features must be in 1..%d" % ops.LAYER_NORM_MAX_COLS)
+        self.features, self.eps = features, eps
+        self.weight = nn.Parameter(torch.ones(features)) if elementwise_affine else None
+        self.bias = nn.Parameter(torch.zeros(features)) if elementwise_affine and bias else None
+
+    def forward(self, x):
+        if x.shape[-1] != self.features:
+            raise ValueError("LayerNorm(%d) got rows of %d elements" % (self.features, x.shape[-1]))
+        return _LayerNormFn.apply(x, self.weight, self.bias, self.eps)
+
+
+# ------------------------------------------------------------------------------------------------------------------
+class _PolicyLossFn(torch.autograd.Function):
+    """The gradient is formed in the backward pass (one more read of the logits): a training step that calls
+    ops.policy_loss(..., dlogits=...) instead gets it from the same read."""
+
+    @staticmethod
+    def forward(ctx, logits, target, advantage, weight, old_logp, ref_logp, clip, kl_coef, inv_tau):
+        need_cuda(logits, "policy_loss")
+        logits = _packed(logits)
+        loss, logp, stats, coef = ops.policy_loss(logits, target, advantage, weight, old_logp=old_logp, ref_logp=ref_logp,
+                                                  clip=clip, kl_coef=kl_coef, inv_tau=inv_tau, save=True)
+        ctx.save_for_backward(logits, target, weight, stats, coef)
+        ctx.inv_tau = inv_tau
+        ctx.mark_non_differentiable(logp)
+        return loss.view(()), logp
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss, _dlogp):
+        logits, target, weight, stats, coef = ctx.saved_tensors
+        d = ops.token_logp_bwd(logits, target, stats, coef, weight=weight, inv_tau=ctx.inv_tau, scale=_packed(dloss))
+        return (d,) + (None,) * 8
+
+
+def policy_loss(logits, target, advantage, weight=None, *, old_logp=None, ref_logp=None, clip=(0.2, 0.2), kl_coef=0.0,
+                inv_tau=1.0):
+    """Clipped policy loss with a KL term (ops.policy_loss), differentiable in `logits` alone: (loss, logp)."""
+    return _PolicyLossFn.apply(logits, target, advantage, weight, old_logp, ref_logp, clip, kl_coef, inv_tau)
+
+
+class _PreferenceLossFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, target, weight, ref_logp, beta, label_smoothing, inv_tau):
+        need_cuda(logits, "preference_loss")
+        logits = _packed(logits)
+        loss, margin, seq_logp, stats, coef = ops.preference_loss(logits, target, weight, ref_logp, beta=beta,
+                                                                  label_smoothing=label_smoothing, inv_tau=inv_tau,
+                                                                  save=True)
+        ctx.save_for_backward(logits, target, weight, stats, coef)
+        ctx.inv_tau = inv_tau
+        ctx.mark_non_differentiable(margin, seq_logp)
+        return loss.view(()), margin, seq_logp
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss, _dmargin, _dseq):
+        logits, target, weight, stats, coef = ctx.saved_tensors
+        d = ops.token_logp_bwd(logits, target, stats, coef, weight=weight, inv_tau=ctx.inv_tau, scale=_packed(dloss))
+        return (d,) + (None,) * 6
+
+
+def preference_loss(logits, target, weight, ref_logp, *, beta, label_smoothing=0.0, inv_tau=1.0):
+    """Preference loss over pairs of sentences (ops.preference_loss), differentiable in `logits` alone:
+    (loss, margin, seq_logp)."""
+    return _PreferenceLossFn.apply(logits, target, weight, ref_logp, beta, label_smoothing, inv_tau)
+
+
+# ------------------------------------------------------------------------------------------------------------------
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0):
+    """torch.nn.utils.clip_grad_norm_ over .grad of the parameters, on the device (ops.clip_grad_norm): scales the
+    gradients in place and returns their norm before that, without waiting for it."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.zeros(1)
+    need_cuda(grads[0], "clip_grad_norm_")
+    return ops.clip_grad_norm(grads, max_norm, norm_type)

@@ -929,13 +929,21 @@ def incr(counter):
     _call("cgn_incr_i32", counter.device, _ptr(counter))
 
 
-def adam(p, g, m, v, lr, step, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0, dyn_step=None):
+def adam(p, g, m, v, lr, step, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0, dyn_step=None, max_norm=None):
+    """One Adam update of flat arenas. max_norm: clip the (scaled) gradient to that 2-norm on the way in; g itself stays
+    as it is. Returns the norm before clipping (device tensor [1]), None without max_norm."""
     n = p.numel()
     for t, nme in ((p, "p"), (g, "g"), (m, "m"), (v, "v")):
         _chk_f32(t, nme)
         _req(t.is_contiguous() and t.numel() == n, "adam arenas must be contiguous and equally sized")
-    _call("cgn_adam_f32", p.device, _ptr(p), _ptr(g), _ptr(m), _ptr(v), n, lr, beta1, beta2, eps, int(step),
-          _ptr(dyn_step), grad_scale)
+    if max_norm is None:
+        _call("cgn_adam_f32", p.device, _ptr(p), _ptr(g), _ptr(m), _ptr(v), n, lr, beta1, beta2, eps, int(step),
+              _ptr(dyn_step), grad_scale)
+        return None
+    norm, coef = _grad_norm([g], 2.0, grad_scale, max_norm)
+    _call("cgn_adam_clipped_f32", p.device, _ptr(p), _ptr(g), _ptr(m), _ptr(v), n, lr, beta1, beta2, eps, int(step),
+          _ptr(dyn_step), grad_scale, _ptr(coef))
+    return norm
 
 
 def disc_head(feat, W, bias, logits, *, mask=None, y=None, w_ce=0.0, w_ent=0.0, p1=None, dlogits=None, stats=None):
@@ -1418,6 +1426,326 @@ def conv_bwd_dx_dense(Ks, Cos, act, layout, W, dfeat, feat, arg, B, L, E, dx, se
     cptrs = (C.c_void_p * n)(*[t_.data_ptr() for t_ in dcols])
     Karr = (C.c_int32 * n)(*Ks)
     _call("cgn_conv_col2im_f32", dev, n, cptrs, Karr, B, L, E, _ptr(dx), sent_stride)
+
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# layer norm (csrc/layernorm.hip)
+# ------------------------------------------------------------------------------------------------------------------
+LAYER_NORM_MAX_COLS = 8192
+
+
+def _rows_any(t, name):
+    """(bf16?, rows, columns, row stride) of a float32 / bfloat16 tensor seen as rows of its last axis: 2-D with unit
+    column stride, or contiguous with any number of axes."""
+    b16 = _chk_f32_or_bf16(t, name)
+    if t.dim() == 2:
+        R, C_ = t.shape
+        ld = t.stride(0) if R > 1 else C_
+        _req((t.stride(1) == 1 or C_ == 1) and ld >= C_, "%s must have unit column stride and rows that do not overlap" % name)
+        return b16, R, C_, ld
+    _req(t.dim() >= 1 and t.is_contiguous(), "%s must be 2-D with unit column stride, or contiguous" % name)
+    C_ = t.shape[-1]
+    return b16, (t.numel() // C_ if C_ else 0), C_, C_
+
+
+def _vector(t, n, name, dev):
+    _chk_f32(t, name)
+    _req(t.numel() == n and t.is_contiguous() and t.device == dev, "%s must be contiguous with %d elements" % (name, n))
+
+
+def _layer_norm_rows(x, name):
+    b16, R, Cn, ld = _rows_any(x, name)
+    _req(1 <= Cn <= LAYER_NORM_MAX_COLS, "layer norm takes rows of 1..%d elements" % LAYER_NORM_MAX_COLS)
+    return b16, R, Cn, ld
+
+
+def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5, out=None):
+    """Layer norm over the last axis: (y, mean, rstd) with y in x's type and shape, mean / rstd float32, one per row.
+    x: float32 or bfloat16, 2-D with any row stride, or contiguous; weight / bias: float32 [C] or None. out: y's
+    destination (x itself is allowed)."""
+    b16, R, Cn, ld = _layer_norm_rows(x, "x")
+    dev = x.device
+    for t, n in ((weight, "weight"), (bias, "bias")):
+        if t is not None:
+            _vector(t, Cn, n, dev)
+    _req(eps >= 0.0, "eps must not be negative")
+    y = alloc(x.shape, dev, x.dtype) if out is None else out
+    _req(y.shape == x.shape and y.dtype == x.dtype and y.device == dev, "out must be like x")
+    ldy = _rows_any(y, "out")[3]
+    stat = alloc((2, R), dev)
+    mean, rstd = stat[0], stat[1]
+    _call("cgn_layer_norm_fwd", dev, _ptr(x), ld, R, Cn, b16, _ptr(weight), _ptr(bias), eps, _ptr(y), ldy, _ptr(mean),
+          _ptr(rstd))
+    return y, mean, rstd
+
+
+def layer_norm_bwd(dy, x, weight, mean, rstd, dx=None, dweight=None, dbias=None, beta=0.0, params=True):
+    """Backward of layer_norm_fwd: (dx, dweight, dbias). dx: its destination (dy's or x's own buffer is allowed), None for
+    a new tensor, False to leave it out. params: form dweight / dbias (= beta * what they hold + the sums over the rows
+    where destinations are given; dweight is None for weight None)."""
+    b16, R, Cn, ldx = _layer_norm_rows(x, "x")
+    dev = x.device
+    _req(dy.shape == x.shape and dy.dtype == x.dtype and dy.device == dev, "dy must be like x")
+    lddy = _rows_any(dy, "dy")[3]
+    for t, n, ne in ((mean, "mean", R), (rstd, "rstd", R)):
+        _vector(t, ne, n, dev)
+    if weight is not None:
+        _vector(weight, Cn, "weight", dev)
+    lddx = Cn
+    if dx is False:
+        dx = None
+    else:
+        dx = alloc(x.shape, dev, x.dtype) if dx is None else dx
+        _req(dx.shape == x.shape and dx.dtype == x.dtype and dx.device == dev, "dx must be like x")
+        lddx = _rows_any(dx, "dx")[3]
+    ws = None
+    if params:
+        _req(beta == 0.0 or dbias is not None, "beta needs destinations that hold something")
+        if dweight is None and weight is not None:
+            _req(beta == 0.0, "beta needs destinations that hold something")
+            dweight = alloc((Cn,), dev)
+        if dbias is None:
+            dbias = alloc((Cn,), dev)
+        for t, n in ((dweight, "dweight"), (dbias, "dbias")):
+            if t is not None:
+                _vector(t, Cn, n, dev)
+        ws = alloc((min(R, 512) * 2 * Cn,), dev)
+    else:
+        _req(dweight is None and dbias is None, "params=False takes no destinations for the parameters")
+    _call("cgn_layer_norm_bwd", dev, _ptr(dy), lddy, _ptr(x), ldx, R, Cn, b16, _ptr(weight), _ptr(mean), _ptr(rstd),
+          _ptr(dx), lddx, _ptr(dweight), _ptr(dbias), float(beta), _ptr(ws), ws.numel() * 4 if ws is not None else 0)
+    return dx, dweight, dbias
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# losses over sampled tokens (csrc/token_loss.hip)
+# ------------------------------------------------------------------------------------------------------------------
+def _token_rows(logits, target, weight, inv_tau, dyn):
+    b16 = _chk_f32_or_bf16(logits, "logits")
+    _chk_i64(target, "target")
+    _req(logits.dim() == 2 and logits.shape[1] > 0 and (logits.stride(1) == 1 or logits.shape[1] == 1),
+         "logits must be [M,V] with unit column stride")
+    M, V = logits.shape
+    ld = logits.stride(0) if M > 1 else V
+    _req(ld >= V, "rows of logits must not overlap")
+    dev = logits.device
+    _req(target.numel() == M and target.device == dev, "target must have M elements")
+    if weight is not None:
+        _vector(weight, M, "weight", dev)
+    if dyn is not None:
+        _chk_f32(dyn, "dyn")
+        _req(dyn.numel() >= 1 and dyn.device == dev, "dyn must hold inv_tau")
+    inv_tau = float(inv_tau)
+    _req(0.0 < inv_tau < float("inf"), "inv_tau must be positive")
+    r = _lib.TokenRows()
+    r.logits, r.ld, r.M, r.target = logits.data_ptr(), ld, M, target.data_ptr()
+    r.weight = weight.data_ptr() if weight is not None else None
+    r.dyn_inv_tau = dyn.data_ptr() if dyn is not None else None
+    r.V, r.bf16, r.inv_tau = V, b16, inv_tau
+    return r, M, V, ld, dev
+
+
+def _dlogits_dest(logits, ld, dlogits):
+    """Row stride of the gradient's destination: a matrix of its own, or exactly the logits' buffer."""
+    M, V = logits.shape
+    _req(isinstance(dlogits, torch.Tensor) and dlogits.shape == logits.shape and dlogits.dtype == logits.dtype
+         and dlogits.device == logits.device and (dlogits.stride(1) == 1 or V == 1),
+         "dlogits must be like logits, with unit column stride")
+    ldd = dlogits.stride(0) if M > 1 else V
+    _req(ldd >= V, "rows of dlogits must not overlap")
+    a, b, size = logits.data_ptr(), dlogits.data_ptr(), logits.element_size()
+    if M and not (a == b and ld == ldd):
+        _req(a + ((M - 1) * ld + V) * size <= b or b + ((M - 1) * ldd + V) * size <= a,
+             "dlogits must be the logits' own buffer or lie apart from it")
+    return ldd
+
+
+def token_logp(logits, target, weight=None, inv_tau=1.0, dyn=None):
+    """(logp, stats): log softmax(inv_tau * logits)[target] for every row of logits [M,V] (float32 or bfloat16, any row
+    stride), and the row statistics token_logp_bwd takes. Rows of weight zero are not read and give 0. dyn: device tensor
+    whose first element overrides inv_tau (graph replay)."""
+    r, M, V, ld, dev = _token_rows(logits, target, weight, inv_tau, dyn)
+    logp, stats = alloc((M,), dev), alloc((M, 2), dev)
+    _call("cgn_token_logp", dev, C.byref(r), _ptr(logp), _ptr(stats))
+    return logp, stats
+
+
+def token_logp_bwd(logits, target, stats, coef, weight=None, inv_tau=1.0, dyn=None, scale=None, dlogits=None):
+    """dlogits[i] = scale * coef[i] * d logp[i] / d logits[i] in logits' type; zeros in rows of weight zero. scale: one
+    float32 on the device, or None. dlogits: the destination (the logits' own buffer is allowed)."""
+    r, M, V, ld, dev = _token_rows(logits, target, weight, inv_tau, dyn)
+    _vector(stats, 2 * M, "stats", dev)
+    _vector(coef, M, "coef", dev)
+    if scale is not None:
+        _vector(scale, 1, "scale", dev)
+    if dlogits is None:
+        dlogits = alloc((M, V), dev, logits.dtype)
+    ldd = _dlogits_dest(logits, ld, dlogits)
+    _call("cgn_token_logp_bwd", dev, C.byref(r), _ptr(stats), _ptr(coef), _ptr(scale), _ptr(dlogits), ldd)
+    return dlogits
+
+
+def policy_loss(logits, target, advantage, weight=None, *, old_logp=None, ref_logp=None, clip=(0.2, 0.2), kl_coef=0.0,
+                inv_tau=1.0, dyn=None, dlogits=None, save=False):
+    """Clipped policy loss with a KL term over sampled tokens: (loss [1], logp [M]), and with `dlogits` its gradient.
+      rho = exp(logp - old_logp) (None: the tokens were drawn from these very logits, rho = 1)
+      loss = sum_i weight_i (-min(rho A, clip(rho, 1 - clip[0], 1 + clip[1]) A) + kl_coef (exp(k) - k - 1)),
+      k = ref_logp - logp
+    logits [M,V] float32 or bfloat16; target int64 [M]; advantage, weight (None: ones), old_logp, ref_logp float32 [M].
+    Rows of weight zero are not read and contribute nothing. For the mean over the tokens that count, divide the weights
+    by their sum. dlogits: destination of d loss / d logits (the logits' own buffer is allowed).
+    save: also return (stats, coef) for token_logp_bwd."""
+    r, M, V, ld, dev = _token_rows(logits, target, weight, inv_tau, dyn)
+    _vector(advantage, M, "advantage", dev)
+    lo, hi, kl_coef = float(clip[0]), float(clip[1]), float(kl_coef)
+    _req(0.0 <= lo < float("inf") and 0.0 <= hi < float("inf"), "clip bounds must not be negative")
+    _req(kl_coef == 0.0 or ref_logp is not None, "kl_coef needs ref_logp")
+    for t, n in ((old_logp, "old_logp"), (ref_logp, "ref_logp")):
+        if t is not None:
+            _vector(t, M, n, dev)
+    ldd = 0 if dlogits is None else _dlogits_dest(logits, ld, dlogits)
+    loss, logp = alloc((1,), dev), alloc((M,), dev)
+    stats, coef = (alloc((M, 2), dev), alloc((M,), dev)) if save else (None, None)
+    ws = alloc((3 * M + 2,), dev, torch.float64)
+    _call("cgn_policy_loss", dev, C.byref(r), _ptr(advantage), _ptr(old_logp), _ptr(ref_logp if kl_coef else None), lo, hi,
+          kl_coef, _ptr(loss), _ptr(logp), _ptr(stats), _ptr(coef), _ptr(dlogits), ldd, _ptr(ws), ws.numel() * 8)
+    return (loss, logp, stats, coef) if save else (loss, logp)
+
+
+def preference_loss(logits, target, weight, ref_logp, *, beta, label_smoothing=0.0, inv_tau=1.0, dyn=None, dlogits=None,
+                    save=False):
+    """Preference loss over pairs of sentences: (loss [1], margin [P], seq_logp [2P]), and with `dlogits` its gradient.
+      S_j = sum_t weight[j,t] logp,  margin_p = beta ((S_p - ref_logp[p]) - (S_{P+p} - ref_logp[P+p]))
+      loss = mean_p -(1 - label_smoothing) log sigmoid(margin_p) - label_smoothing log sigmoid(-margin_p)
+    weight: float32 [2P, T]; sentences 0..P-1 are the preferred ones, P..2P-1 the others of the same pairs; logits
+    [2P*T, V] and target [2P*T] hold their rows sentence by sentence; tokens of weight zero (padding) are not read.
+    ref_logp: float32 [2P], the sentences' log-probabilities under the reference model. dlogits, save: as policy_loss."""
+    r, M, V, ld, dev = _token_rows(logits, target, weight, inv_tau, dyn)
+    _req(weight is not None and weight.dim() == 2 and weight.shape[0] % 2 == 0 and M > 0,
+         "weight must be [2P,T] with P, T >= 1")
+    S, T = weight.shape
+    _vector(ref_logp, S, "ref_logp", dev)
+    beta, label_smoothing = float(beta), float(label_smoothing)
+    _req(0.0 < beta < float("inf") and 0.0 <= label_smoothing < 0.5, "beta > 0 and 0 <= label_smoothing < 0.5")
+    ldd = 0 if dlogits is None else _dlogits_dest(logits, ld, dlogits)
+    loss, margin, seq_logp = alloc((1,), dev), alloc((S // 2,), dev), alloc((S,), dev)
+    stats, coef = (alloc((M, 2), dev), alloc((M,), dev)) if save else (None, None)
+    ws = alloc((3 * M + 2,), dev, torch.float64)
+    _call("cgn_preference_loss", dev, C.byref(r), T, _ptr(ref_logp), beta, label_smoothing, _ptr(loss), _ptr(margin),
+          _ptr(seq_logp), _ptr(stats), _ptr(coef), _ptr(dlogits), ldd, _ptr(ws), ws.numel() * 8)
+    return (loss, margin, seq_logp, stats, coef) if save else (loss, margin, seq_logp)
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# global gradient norm and clipping (csrc/gradnorm.hip)
+# ------------------------------------------------------------------------------------------------------------------
+def _grad_layout(t):
+    """(rows, columns, row stride): one piece of memory, or a matrix with a row stride (the arenas' padded views)."""
+    if t.is_contiguous():
+        return 1, t.numel(), 0
+    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1]:
+        return t.shape[0], t.shape[1], t.stride(0)
+    n = 1
+    for st, sz in sorted(zip(t.stride(), t.shape)):  # a permuted view of one piece
+        if sz != 1 and st != n:
+            raise ValueError("a gradient must be one piece of memory or a matrix with unit column stride, got %s / %s"
+                             % (tuple(t.shape), t.stride()))
+        n *= sz
+    return 1, t.numel(), 0
+
+
+def _grad_table(grads, out):
+    """cgn_grad_tensor table of a list of gradients (and their destinations), checked on the host."""
+    flat, spans = [], []
+    dev = grads[0].device
+    for i, g in enumerate(grads):
+        b16 = _chk_f32_or_bf16(g, "grads[%d]" % i)
+        if g.device != dev:
+            raise ValueError("gradients on different devices")
+        rows, cols, ld = _grad_layout(g)
+        p = g.data_ptr()
+        if out is None:
+            flat += (p, p, rows, cols, ld, ld, b16)
+            continue
+        o = out[i]
+        q, ldo = p, ld
+        if o is not g:
+            _req(isinstance(o, torch.Tensor) and o.shape == g.shape and o.dtype == g.dtype and o.device == dev,
+                 "out[%d] must be like its gradient" % i)
+            orows, _, ldo = _grad_layout(o)
+            _req(orows == rows and (rows > 1 or o.stride() == g.stride() or (o.is_contiguous() and g.is_contiguous())),
+                 "out[%d] must be laid out like its gradient" % i)
+            q = o.data_ptr()
+        flat += (p, q, rows, cols, ld, ldo, b16)
+        if rows and cols:
+            size = 2 if b16 else 4
+            spans.append((q, q + ((rows - 1) * ldo + cols) * size))
+            if q != p or ldo != ld:
+                spans.append((p, p + ((rows - 1) * ld + cols) * size))
+    if out is not None:
+        spans.sort()
+        end = 0
+        for a, b in spans:
+            if a < end:
+                raise ValueError("gradients to be clipped must not overlap in memory (the same tensor twice?)")
+            end = b
+    return (C.c_int64 * len(flat))(*flat), len(grads), dev
+
+
+def _norm_kind(norm_type):
+    norm_type = float(norm_type)
+    _req(norm_type in (2.0, float("inf")), "norm_type must be 2 or inf")
+    return 1 if norm_type != 2.0 else 0
+
+
+def _grad_list(grads):
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    _req(len(grads) > 0, "no gradients given")
+    return grads
+
+
+def _norm_workspace(table, n, dev):
+    nb = C.c_int64()
+    _lib.check(_lib.load().cgn_grad_norm_workspace(table, n, C.byref(nb)), "cgn_grad_norm_workspace")
+    return alloc((nb.value // 8,), dev, torch.float64)
+
+
+def _grad_norm(grads, norm_type, grad_scale, max_norm):
+    kind = _norm_kind(norm_type)
+    max_norm = float(max_norm)
+    _req(max_norm >= 0.0, "max_norm must not be negative")
+    table, n, dev = _grad_table(grads, None)
+    ws = _norm_workspace(table, n, dev)
+    res = alloc((2,), dev)
+    norm, coef = res[:1], res[1:]
+    _call("cgn_grad_norm", dev, table, n, kind, float(grad_scale), max_norm, _ptr(norm), _ptr(coef), _ptr(ws),
+          ws.numel() * 8)
+    return norm, coef
+
+
+def grad_norm(grads, norm_type=2.0, grad_scale=1.0):
+    """Norm of all elements of a list of tensors (float32 / bfloat16, mixed) taken as one vector, times |grad_scale|:
+    device tensor [1]. norm_type 2 or inf. A tensor is one piece of memory or a matrix with a row stride. The squares are
+    summed in 64 bits; nothing is read back to the host."""
+    return _grad_norm(_grad_list(grads), norm_type, grad_scale, 0.0)[0]
+
+
+def clip_grad_norm(grads, max_norm, norm_type=2.0, out=None, grad_scale=1.0):
+    """Scale a list of gradients by grad_scale * min(1, max_norm / (norm + 1e-6)), norm = grad_norm(grads, norm_type,
+    grad_scale): in place, or into the tensors of `out`. Returns the norm before clipping (device tensor [1]). The tensors
+    must not overlap in memory. A NaN among the gradients makes all of them NaN, as the formula says."""
+    grads = _grad_list(grads)
+    kind = _norm_kind(norm_type)
+    max_norm = float(max_norm)
+    _req(max_norm >= 0.0, "max_norm must not be negative")
+    out = grads if out is None else ([out] if isinstance(out, torch.Tensor) else list(out))
+    _req(len(out) == len(grads), "one destination per gradient")
+    table, n, dev = _grad_table(grads, out)
+    ws = _norm_workspace(table, n, dev)
+    norm = alloc((1,), dev)
+    _call("cgn_clip_grads", dev, table, n, kind, float(grad_scale), max_norm, _ptr(norm), _ptr(ws), ws.numel() * 8)
+    return norm
 
 
 if COMPUTE == _lib.COMPUTE_BF16:

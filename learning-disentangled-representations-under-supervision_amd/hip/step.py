@@ -92,6 +92,10 @@ class CGNStep:
         self.allreduce = allreduce
         self.world_size = world_size
         self.dp = allreduce is not None and (world_size > 1 or force_dp)
+        # bound on the 2-norm of every optimizer group's gradient (averaged over the ranks), None = no clipping (the
+        # reference's behaviour); the last step's norms before clipping are in `grad_norms`, by group, as device tensors
+        self.max_grad_norm = None
+        self.grad_norms = {}
         self._pending = {}     # optimizer group -> handles of its gradient all-reduce in flight
         # The encoder group's gradients become final in two waves: the biLSTM's and the mu|logvar head's right behind the
         # LSTM backward (side stream 0), the highway's, the TDNN's and the char table's only at the very end of the step.
@@ -256,7 +260,10 @@ class CGNStep:
         return self.arenas[group].new_adam()
 
     def _adam(self, state):
-        state.apply(self.cfg.learning_rate, grad_scale=1.0 / self.world_size, dynamic=self.dynamic)
+        norm = state.apply(self.cfg.learning_rate, grad_scale=1.0 / self.world_size, dynamic=self.dynamic,
+                           max_norm=self.max_grad_norm)
+        if norm is not None:
+            self.grad_norms[state.arena.group] = norm
 
     def _optim_step(self, state):
         if self.dp:

@@ -1,0 +1,810 @@
+"""Tuning operators on the GPU against their formulas in 64 bits: layer norm, log-probabilities of sampled tokens, the
+clipped policy loss, the preference loss, the global gradient norm and clipping.
+
+Tolerances count roundings. u = 2^-24 is half a step of fp32, eps/2 half a step of the output's type. The longest chain of
+fp32 additions in a sum is 32 terms in a thread plus 10 levels of a tree (see the kernels), so a sum of n terms of either
+sign is off by at most 42 u sum|term|; the handful of further operations per element is rounded up to 64 u in all."""
+import math
+
+import pytest
+import torch
+
+import ldrs_amd  # noqa: F401
+from ldrs_amd.hip import nn as hnn
+from ldrs_amd.hip import ops
+from ldrs_amd.hip.arena import ParamArena
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def half(t):
+    return torch.finfo(t.dtype).eps / 2
+
+
+def close(got, want, tol, what):
+    """|got - want| <= tol elementwise, `got` rounded once from a value inside that band."""
+    got, want = got.double(), want.double()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    bad = ~((got - want).abs() <= tol)
+    assert not bad.any(), (what, int(bad.sum()), float((got - want).abs()[bad].max()))
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def strided(t, extra, shift=0):
+    """The same matrix inside a wider buffer: row stride shape[1] + extra, starting `shift` elements in."""
+    R, C = t.shape
+    buf = torch.full((R * (C + extra) + shift + 8,), float("nan"), dtype=t.dtype, device=t.device)
+    v = buf[shift:shift + R * (C + extra)].view(R, C + extra)[:, :C]
+    v.copy_(t)
+    return v
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# layer norm
+# ---------------------------------------------------------------------------------------------------------------------
+def norm_ref(x, w, b, eps, dy=None):
+    x = x.double()
+    w = torch.ones(x.shape[-1], dtype=torch.float64, device=x.device) if w is None else w.double()
+    b = torch.zeros_like(w) if b is None else b.double()
+    mu = x.mean(-1, keepdim=True)
+    r = 1.0 / torch.sqrt(((x - mu) ** 2).mean(-1, keepdim=True) + eps)
+    xh = (x - mu) * r
+    out = dict(mu=mu[:, 0], r=r[:, 0], xh=xh, y=xh * w + b)
+    if dy is not None:
+        dy = dy.double()
+        g = dy * w
+        mg, mgx = g.mean(-1, keepdim=True), (g * xh).mean(-1, keepdim=True)
+        out.update(dx=r * (g - mg - xh * mgx), dw=(dy * xh).sum(0), db=dy.sum(0))
+        out["dx_tol"] = 128 * U * r * (g.abs() + g.abs().mean(-1, keepdim=True)
+                                       + (xh.abs() + 1) * (g * xh).abs().mean(-1, keepdim=True))
+        # 128 u also covers the additions over the rows: at most 41 in a lane (R <= 21000 in 512 workgroups), the
+        # workgroup's groups (32) and the reduction over the workgroups (32 + 16)
+        out["dw_tol"] = 128 * U * (dy.abs() * (xh.abs() + 1)).sum(0)
+        out["db_tol"] = 128 * U * dy.abs().sum(0)
+    return out
+
+
+NORM_SIZES = [(1, 1), (3, 1), (1, 2), (5, 7), (2, 8), (33, 9), (64, 33), (7, 63), (9, 64), (4, 65), (130, 127), (3, 256),
+              (5, 257), (3, 300), (65, 512), (6, 513), (4, 600), (10, 800), (37, 825), (300, 1024), (5, 1025), (2, 2047),
+              (3, 2049), (2, 4096), (3, 4097), (2, 8191), (2, 8192), (2100, 40)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("R,C", NORM_SIZES)
+def test_layer_norm(dev, R, C, dtype):
+    g = gen(R * 10007 + C)
+    x = (torch.randn(R, C, device=dev, generator=g) * 2 + torch.randn(R, 1, device=dev, generator=g)).to(dtype)
+    dy = torch.randn(R, C, device=dev, generator=g).to(dtype)
+    w, b = torch.randn(C, device=dev, generator=g), torch.randn(C, device=dev, generator=g)
+    ref = norm_ref(x, w, b, 1e-5, dy)
+    y, mean, rstd = ops.layer_norm_fwd(x, w, b, 1e-5)
+    assert y.dtype == dtype and mean.shape == rstd.shape == (R,)
+    close(mean, ref["mu"], 42 * U * x.double().abs().mean(-1), "mean")
+    close(rstd, ref["r"], 64 * U * ref["r"], "rstd")
+    ytol = 64 * U * (ref["xh"].abs() * w.abs() + w.abs() + b.abs())
+    close(y, ref["y"], ytol + half(y) * (ref["y"].abs() + ytol), "y")
+    dx, dw, db = ops.layer_norm_bwd(dy, x, w, mean, rstd)
+    close(dx, ref["dx"], ref["dx_tol"] + half(dx) * (ref["dx"].abs() + ref["dx_tol"]), "dx")
+    close(dw, ref["dw"], ref["dw_tol"], "dweight")
+    close(db, ref["db"], ref["db_tol"], "dbias")
+    again = ops.layer_norm_bwd(dy, x, w, mean, rstd)
+    assert all(torch.equal(p, q) for p, q in zip((dx, dw, db), again)), "two runs, two answers"
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("C,extra,shift", [(300, 4, 0), (257, 3, 1), (825, 0, 3), (64, 1, 5), (2049, 7, 1)])
+def test_layer_norm_strides_in_place_and_optional_parts(dev, C, extra, shift, dtype):
+    R, g = 21, gen(C)
+    x0 = torch.randn(R, C, device=dev, generator=g).to(dtype)
+    dy0 = torch.randn(R, C, device=dev, generator=g).to(dtype)
+    w = torch.randn(C, device=dev, generator=g)
+    y0, mean, rstd = ops.layer_norm_fwd(x0, w, None, 1e-5)
+    d0 = ops.layer_norm_bwd(dy0, x0, w, mean, rstd)
+    x, dy, y, dx = (strided(t, extra, shift) for t in (x0, dy0, x0, x0))
+    assert ops.layer_norm_fwd(x, w, None, 1e-5, out=y)[0] is y and torch.equal(y, y0)
+    got = ops.layer_norm_bwd(dy, x, w, mean, rstd, dx=dx)
+    assert got[0] is dx and all(torch.equal(p, q) for p, q in zip(got, d0))
+    for t in (y, dx):  # nothing beside the rows was written
+        flat = t.as_strided((R * (C + extra) + 8,), (1,), t.storage_offset())
+        pad = torch.cat([flat[r * (C + extra) + C:(r + 1) * (C + extra)] for r in range(R)] + [flat[R * (C + extra):]])
+        assert pad.isnan().all()
+    # in place: y over x, dx over dy, dx over x
+    xi = strided(x0, extra, shift)
+    assert torch.equal(ops.layer_norm_fwd(xi, w, None, 1e-5, out=xi)[0], y0)
+    for over in (0, 1):
+        di, xi = strided(dy0, extra, shift), strided(x0, extra, shift)
+        assert torch.equal(ops.layer_norm_bwd(di, xi, w, mean, rstd, dx=(di, xi)[over])[0], d0[0])
+    # parts alone, and accumulation into gradients that are there
+    assert torch.equal(ops.layer_norm_bwd(dy0, x0, w, mean, rstd, params=False)[0], d0[0])
+    only = ops.layer_norm_bwd(dy0, x0, w, mean, rstd, dx=False)
+    assert only[0] is None and torch.equal(only[1], d0[1]) and torch.equal(only[2], d0[2])
+    aw, ab = torch.randn(C, device=dev, generator=g), torch.randn(C, device=dev, generator=g)
+    want = (aw * 0.5 + d0[1], ab * 0.5 + d0[2])
+    ops.layer_norm_bwd(dy0, x0, w, mean, rstd, dx=False, dweight=aw, dbias=ab, beta=0.5)
+    for p, q in zip((aw, ab), want):
+        close(p, q, 2 * U * (q.double().abs() + p.double().abs() + 1), "beta")
+    # no parameters at all
+    ref = norm_ref(x0, None, None, 0.0, dy0)
+    y, mean, rstd = ops.layer_norm_fwd(x0, eps=0.0)
+    ytol = 64 * U * (ref["xh"].abs() + 1)
+    close(y, ref["y"], ytol + half(y) * (ref["y"].abs() + ytol), "y without parameters")
+    dx, dw, db = ops.layer_norm_bwd(dy0, x0, None, mean, rstd)
+    assert dw is None
+    close(dx, ref["dx"], ref["dx_tol"] + half(dx) * (ref["dx"].abs() + ref["dx_tol"]), "dx without parameters")
+
+
+def test_layer_norm_keeps_precision_far_from_zero(dev):
+    """A row's mean 1000 times its spread: the statistics' second sum takes out what the first one's rounding left."""
+    g = gen(5)
+    x = torch.randn(40, 825, device=dev, generator=g) + 1000.0
+    dy = torch.randn(40, 825, device=dev, generator=g)
+    ref = norm_ref(x, None, None, 1e-5, dy)
+    y, mean, rstd = ops.layer_norm_fwd(x)
+    close(y, ref["y"], 64 * U * (ref["xh"].abs() + 1), "y")
+    dx = ops.layer_norm_bwd(dy, x, None, mean, rstd)[0]
+    close(dx, ref["dx"], ref["dx_tol"], "dx")
+
+
+def test_layer_norm_no_rows_and_special_values(dev):
+    w = torch.ones(12, device=dev)
+    y, mean, rstd = ops.layer_norm_fwd(torch.empty(0, 12, device=dev), w)
+    assert y.shape == (0, 12) and mean.numel() == 0
+    dx, dw, db = ops.layer_norm_bwd(y, y, w, mean, rstd)
+    assert dx.shape == (0, 12) and not dw.any() and not db.any()
+    x = torch.randn(4, 12, device=dev)
+    x[1, 3], x[2, 5] = float("nan"), float("inf")
+    y = ops.layer_norm_fwd(x, w)[0]
+    assert y[1].isnan().all() and y[2].isnan().any() and torch.isfinite(y[[0, 3]]).all()
+    y, _, rstd = ops.layer_norm_fwd(torch.full((2, 12), 3.0, device=dev), w, w)  # no spread at all: the bias is left
+    assert torch.equal(y, torch.ones_like(y)) and torch.allclose(rstd, torch.full_like(rstd, 1e-5 ** -0.5))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_layer_norm_module(dev, dtype):
+    """The nn module: leading axes, an expanded gradient, partial requires_grad; its gradients against differences."""
+    g = gen(3)
+    m = hnn.LayerNorm(50).to(dev)
+    with torch.no_grad():
+        m.weight.copy_(torch.randn(50, device=dev, generator=g))
+        m.bias.copy_(torch.randn(50, device=dev, generator=g))
+    x = torch.randn(3, 5, 50, device=dev, generator=g).to(dtype).requires_grad_()
+    y = m(x)
+    assert y.shape == x.shape and y.dtype == dtype
+    y.sum().backward()  # an expanded dy of ones
+    ref = norm_ref(x.detach().view(15, 50), m.weight.detach(), m.bias.detach(), m.eps, torch.ones(15, 50, device=dev))
+    close(x.grad.view(15, 50), ref["dx"], ref["dx_tol"] + half(x) * (ref["dx"].abs() + ref["dx_tol"]), "dx")
+    close(m.weight.grad, ref["dw"], ref["dw_tol"], "dweight")
+    close(m.bias.grad, ref["db"], ref["db_tol"], "dbias")
+    x2 = x.detach().transpose(0, 1)  # not contiguous, no gradient wanted for it
+    m.zero_grad()
+    m(x2).float().square().sum().backward()
+    assert m.weight.grad is not None and x2.grad is None
+    if dtype == F32:  # directional derivative by central differences, in fp32 arithmetic on both sides
+        xd = x.detach().clone().requires_grad_()
+        c, v = torch.randn(3, 5, 50, device=dev, generator=g), torch.randn(3, 5, 50, device=dev, generator=g)
+        (m(xd) * c).sum().backward()
+        h = 2.0 ** -8
+        with torch.no_grad():
+            num = ((m(xd + h * v).double() - m(xd - h * v).double()) * c.double()).sum() / (2 * h)
+        # truncation h^2/6 f''' with |f'''| of the order of |c||v|^3, rounding 64 u |y||c| / h
+        scale = float((c.double().abs() * (1 + v.double().abs()) ** 3).sum())
+        assert abs(float(num) - float((xd.grad.double() * v.double()).sum())) <= scale * (8 * h * h + 64 * U / h)
+    nb = hnn.LayerNorm(50, elementwise_affine=False).to(dev)
+    assert torch.equal(nb(x.detach()), ops.layer_norm_fwd(x.detach())[0])
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# losses over sampled tokens
+# ---------------------------------------------------------------------------------------------------------------------
+def make_rows(M, V, dtype, seed, dev, spread=3.0):
+    g = gen(seed)
+    x = (torch.randn(M, V, device=dev, generator=g) * spread).to(dtype)
+    t = torch.randint(0, V, (M,), device=dev, generator=g)
+    best = x.float().argmax(1)
+    t = torch.where(torch.rand(M, device=dev, generator=g) < 0.5, best, t)
+    return x, t, g
+
+
+def softmax_ref(x, t, it):
+    """Log-probabilities of the targets, probabilities and the band of a log-probability: v_exp_f32's and the argument's
+    roundings (2 u |log p|, at most ln V + a few on average under the softmax) and the sums' 42 u, twice over."""
+    a = x.double() * it
+    ls = torch.log_softmax(a, 1)
+    lp = ls.gather(1, t[:, None])[:, 0]
+    return lp, ls, 128 * U + 2 * U * lp.abs()
+
+
+def dlogits_ref(ls, t, coef, it, band, cabs):
+    """coef * it * (1[target] - p) and its band: the coefficient's (cabs times the log-probability's) and the
+    probabilities' own (2 u |log p| + 64 u)."""
+    p = ls.exp()
+    d = -p
+    d[torch.arange(len(t), device=t.device), t] += 1
+    hot = torch.zeros_like(p)
+    hot[torch.arange(len(t), device=t.device), t] = 1
+    size = p * (64 * U + 4 * U * ls.abs().clamp(max=200)) + (p + hot) * 4 * U
+    tol = it * (coef.abs()[:, None] * size + (cabs * (2 * band + 8 * U))[:, None] * (p + hot))
+    return d * (coef * it)[:, None], tol + 1e-36
+
+
+def check_dlogits(got, want, tol, what):
+    close(got, want, tol + half(got) * (want.abs() + tol) + (2.0 ** -133 if got.dtype == BF16 else 0), what)
+
+
+# sizes on both sides of every register variant: pieces of 4 (fp32) / 8 (bf16) elements, 256..1024 threads
+ROW_SIZES = [(1, 1), (5, 2), (3, 7), (4, 8), (7, 9), (2, 1000), (3, 1023), (2, 1024), (2, 1025), (3, 2049), (2, 4097),
+             (2, 8193), (3, 10000), (2, 16385), (2, 20001), (2, 24577), (2, 32769), (1, 49153), (2, 50000), (1, 65537),
+             (1, 98305), (1, 131075)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M,V", ROW_SIZES)
+def test_token_logp(dev, M, V, dtype):
+    x, t, g = make_rows(M, V, dtype, M * 100003 + V, dev)
+    for it in (1.0, 0.7):
+        logp, stats = ops.token_logp(x, t, inv_tau=it)
+        it64 = float(torch.tensor(it, dtype=F32))
+        lp, ls, band = softmax_ref(x, t, it64)
+        close(logp, lp, band, "logp")
+        coef = torch.randn(M, device=dev, generator=g)
+        want, tol = dlogits_ref(ls, t, coef.double(), it64, band, torch.zeros_like(band))
+        d = ops.token_logp_bwd(x, t, stats, coef, inv_tau=it)
+        assert d.dtype == dtype
+        check_dlogits(d, want, tol, "dlogits")
+        scale = torch.tensor([0.25], device=dev)
+        check_dlogits(ops.token_logp_bwd(x, t, stats, coef, inv_tau=it, scale=scale), want / 4, tol / 4, "scaled")
+        dyn = torch.tensor([it], device=dev)
+        assert torch.equal(ops.token_logp(x, t, dyn=dyn)[0], logp)
+        xi = x.clone()
+        assert torch.equal(ops.token_logp_bwd(xi, t, stats, coef, inv_tau=it, dlogits=xi), d)
+
+
+def policy_ref(x, t, A, w, old, ref, lo, hi, kl, it):
+    lp, ls, band = softmax_ref(x, t, it)
+    A, w = A.double(), w.double()
+    rho = torch.ones_like(lp) if old is None else (lp - old.double()).exp()
+    cut = ((A > 0) & (rho > 1 + hi)) | ((A < 0) & (rho < 1 - lo))
+    L = -torch.minimum(rho * A, rho.clamp(1 - lo, 1 + hi) * A)
+    g = -torch.where(cut, 0.0, rho * A)
+    cabs = torch.where(cut, 0.0, (rho * A).abs())
+    if kl:
+        k = ref.double() - lp
+        L = L + kl * (k.exp() - k - 1)
+        g = g + kl * (1 - k.exp())
+        cabs = cabs + kl * (k.exp() + 1)
+    live = w != 0
+    z = torch.zeros_like(lp)
+    out = dict(loss=torch.where(live, w * L, z).sum(), logp=torch.where(live, lp, z), band=band)
+    out["loss_tol"] = float(torch.where(live, (w.abs() * ((rho * A).abs() + (kl * (k.exp() + 1) if kl else 0))
+                                               * (2 * band + 8 * U)), z).sum())
+    coef, cabs = torch.where(live, w * g, z), torch.where(live, w.abs() * cabs, z)
+    out["d"], out["d_tol"] = dlogits_ref(ls, t, coef, it, band, cabs)
+    out["d"][~live] = 0
+    return out
+
+
+def make_policy(M, V, dtype, seed, dev, it=1.0, dead=0.3):
+    x, t, g = make_rows(M, V, dtype, seed, dev)
+    lp = softmax_ref(x, t, it)[0]
+    w = torch.rand(M, device=dev, generator=g) + 0.1
+    if M > 1:
+        w[torch.rand(M, device=dev, generator=g) < dead] = 0
+        w[0] = 0.5
+    d = 0.3 * torch.randn(M, device=dev, generator=g).double()
+    for e in (0.8, 1.3):  # off the two borders, where the gradient jumps
+        d = torch.where((d - math.log(e)).abs() < 1e-3, d + 4e-3, d)
+    old = (lp - d).float()
+    ref = (lp + 0.3 * torch.randn(M, device=dev, generator=g)).float()
+    return x, t, torch.randn(M, device=dev, generator=g), w, old, ref
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M,V", ROW_SIZES + [(40, 333), (300, 77)])
+def test_policy_loss(dev, M, V, dtype):
+    it = 1.25
+    x, t, A, w, old, ref = make_policy(M, V, dtype, M * 31 + V, dev, it)
+    for kl, o in ((0.1, old), (0.0, old), (0.1, None)):
+        want = policy_ref(x, t, A, w, o, ref, 0.2, 0.3, kl, it)
+        d = torch.full_like(x, float("nan"))
+        loss, logp = ops.policy_loss(x, t, A, w, old_logp=o, ref_logp=ref, clip=(0.2, 0.3), kl_coef=kl, inv_tau=it,
+                                     dlogits=d)
+        close(logp, want["logp"], want["band"], "logp")
+        assert abs(float(loss) - float(want["loss"])) <= want["loss_tol"] + 2 * U * abs(float(want["loss"])), "loss"
+        check_dlogits(d, want["d"], want["d_tol"], "dlogits")
+        # without the gradient, over the logits' own buffer, and through the saved statistics: the same numbers
+        loss2, logp2, stats, coef = ops.policy_loss(x, t, A, w, old_logp=o, ref_logp=ref, clip=(0.2, 0.3), kl_coef=kl,
+                                                    inv_tau=it, save=True)
+        assert torch.equal(loss2, loss) and torch.equal(logp2, logp)
+        xi = x.clone()
+        ops.policy_loss(xi, t, A, w, old_logp=o, ref_logp=ref, clip=(0.2, 0.3), kl_coef=kl, inv_tau=it, dlogits=xi)
+        assert torch.equal(xi, d)
+        check_dlogits(ops.token_logp_bwd(x, t, stats, coef, weight=w, inv_tau=it), want["d"], want["d_tol"], "saved")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_policy_loss_is_clipped_where_the_formula_says(dev, dtype):
+    """Ratios 0.5, 1, 2 with advantages of both signs and zero: which of the six are cut, and their losses."""
+    V = 50
+    x, t, _ = make_rows(9, V, dtype, 1, dev)
+    lp = softmax_ref(x, t, 1.0)[0]
+    ratio = torch.tensor([0.5, 1.0, 2.0] * 3, device=dev, dtype=torch.float64)
+    A = torch.tensor([1.0] * 3 + [-1.0] * 3 + [0.0] * 3, device=dev)
+    old = (lp - ratio.log()).float()
+    for i in range(9):
+        w = torch.zeros(9, device=dev)
+        w[i] = 1
+        d = torch.empty_like(x)
+        loss, _ = ops.policy_loss(x, t, A, w, old_logp=old, dlogits=d)
+        want = [-0.5, -1.0, -1.2, 0.8, 1.0, 2.0, 0.0, 0.0, 0.0][i]
+        assert abs(float(loss) - want) <= 1e-5, i
+        moves = i in (0, 1, 4, 5)  # the rest is cut, or has nothing to say
+        assert bool(d[i].any()) == moves and not d[torch.arange(9, device=dev) != i].any(), i
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V,extra,shift", [(333, 5, 0), (1000, 0, 1), (2050, 3, 3), (131080, 1, 1)])
+def test_masked_rows_strides_and_bad_values(dev, V, extra, shift, dtype):
+    """Rows of weight zero hold NaN, infinities, the type's lowest value and targets from nowhere: nothing of it shows."""
+    M, inf = 8, float("inf")
+    x0, t, A, w, old, ref = make_policy(M, V, dtype, V, dev)
+    w[:] = torch.tensor([0.3, 0, 0.2, 0, 0, 0.1, 0, 0], device=dev)
+    d0 = torch.empty_like(x0)
+    loss0, logp0 = ops.policy_loss(x0, t, A, w, old_logp=old, ref_logp=ref, kl_coef=0.1, dlogits=d0)
+    dead = w == 0
+    bad = torch.tensor([0, float("nan"), 0, inf, -inf, 0, torch.finfo(dtype).min, inf], device=dev).to(dtype)
+    x = strided(torch.where(dead[:, None], bad[:, None], x0), extra, shift)
+    t2 = torch.where(dead, torch.tensor([0, -100, 0, V, 1 << 40, 0, -(1 << 60), V + 7], device=dev), t)
+    nan = torch.full_like(A, float("nan"))
+    A2, old2, ref2 = (torch.where(dead, nan, v) for v in (A, old, ref))
+    d = strided(torch.full_like(x0, 7.0), extra, shift)
+    loss, logp = ops.policy_loss(x, t2, A2, w, old_logp=old2, ref_logp=ref2, kl_coef=0.1, dlogits=d)
+    assert torch.equal(loss, loss0) and torch.equal(logp, logp0) and torch.equal(d, d0)
+    assert not d[dead].any() and not logp[dead].any()
+    flat = d.as_strided((M * (V + extra) + 8,), (1,), d.storage_offset())
+    pad = torch.cat([flat[r * (V + extra) + V:(r + 1) * (V + extra)] for r in range(M)] + [flat[M * (V + extra):]])
+    assert pad.isnan().all(), "written beside the rows"
+    # no row left at all
+    loss, logp = ops.policy_loss(x, t2, A2, torch.zeros_like(w), old_logp=old2, dlogits=d)
+    assert float(loss) == 0.0 and not logp.any() and not d.any()
+    # a target outside the vocabulary in a row that counts: NaN, in that row alone
+    t3 = t.clone()
+    t3[2] = V
+    loss, logp = ops.policy_loss(x0, t3, A, w, old_logp=old, dlogits=d)
+    assert loss.isnan().all() and logp[2].isnan() and d[2].isnan().all()
+    assert torch.isfinite(d[[0, 1, 3, 4, 5, 6, 7]].float()).all() and torch.isfinite(logp[[0, 5]]).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [40, 3000, 140000])
+def test_banned_tokens(dev, V, dtype):
+    """-inf and the type's lowest value in rows that count: those tokens have probability and gradient zero."""
+    x, t, A, w, old, ref = make_policy(6, V, dtype, V, dev, dead=0.0)
+    keep = torch.zeros(6, V, dtype=torch.bool, device=dev)
+    keep[torch.arange(6, device=dev), t] = True
+    ban = (torch.rand(6, V, device=dev, generator=gen(9)) < 0.5) & ~keep
+    ban[5] = ~keep[5]  # everything but the target
+    x[ban] = -float("inf")
+    x[:3][ban[:3]] = torch.finfo(dtype).min
+    want = policy_ref(x, t, A, w, None, ref, 0.2, 0.2, 0.0, 1.0)
+    d = torch.empty_like(x)
+    loss, logp = ops.policy_loss(x, t, A, w, dlogits=d)
+    close(logp, want["logp"], want["band"], "logp")
+    assert float(logp[5]) == 0.0 and not d[5].any()
+    assert not d[ban].any() and torch.isfinite(d.float()).all()
+    want["d"][ban], want["d_tol"][ban] = 0, 0
+    check_dlogits(d, want["d"], want["d_tol"], "dlogits")
+    x[1] = -float("inf")  # no token is possible: as log_softmax says, NaN
+    _, logp = ops.policy_loss(x, t, A, w, dlogits=d)
+    assert logp[1].isnan() and d[1].isnan().all() and torch.isfinite(logp[[0, 2, 3, 4, 5]]).all()
+    _, logp = ops.policy_loss(x, t, A, w)
+    assert logp[1].isnan()
+
+
+def pair_ref(x, t, w, ref, beta, smooth, it):
+    P = w.shape[0] // 2
+    lp, ls, band = softmax_ref(x, t, it)
+    w64 = w.double()
+    live = w64 != 0
+    z = torch.zeros_like(w64)
+    S = torch.where(live, w64 * lp.view_as(w64), z).sum(1)
+    dS = torch.where(live, w64.abs() * band.view_as(w64), z).sum(1)
+    gain = S - ref.double()
+    m = beta * (gain[:P] - gain[P:])
+    dm = beta * (dS[:P] + dS[P:])
+    loss = -((1 - smooth) * torch.nn.functional.logsigmoid(m) + smooth * torch.nn.functional.logsigmoid(-m))
+    up = -(beta / P) * ((1 - smooth) * torch.sigmoid(-m) - smooth * torch.sigmoid(m))
+    dup = beta / P * (dm / 4 + 4 * U * up.abs())
+    coef = (torch.cat((up, -up))[:, None] * w64).view(-1)
+    cerr = (torch.cat((dup, dup))[:, None] * w64.abs()).view(-1)
+    d, tol = dlogits_ref(ls, t, coef, it, torch.zeros_like(band), coef.abs() + 1)
+    hot = torch.zeros_like(d)
+    hot[torch.arange(len(t), device=t.device), t] = 1
+    tol = tol + it * (cerr + 4 * U * coef.abs())[:, None] * (ls.exp() + hot)
+    d[~live.view(-1)] = 0
+    return dict(S=S, dS=dS + U * S.abs(), m=m, dm=dm + U * m.abs(), loss=loss.mean(), dl=float(dm.mean()), d=d, tol=tol)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("P,T,V", [(1, 1, 5), (1, 3, 1000), (3, 1, 33), (2, 65, 77), (5, 21, 300), (2, 7, 20001),
+                                   (1, 2, 131075), (70, 3, 40)])
+def test_preference_loss(dev, P, T, V, dtype):
+    x, t, g = make_rows(2 * P * T, V, dtype, P * 1009 + T * 101 + V, dev)
+    n = torch.randint(0, T + 1, (2 * P, 1), device=dev, generator=g)
+    n[0] = T
+    w = (torch.arange(T, device=dev)[None] < n).float() * (1 + torch.rand(2 * P, T, device=dev, generator=g))
+    if P > 1:
+        w[1] = 0  # an empty sentence
+    S = (softmax_ref(x, t, 1.0)[0].view(2 * P, T) * w).sum(1)
+    ref = (S + 5 * torch.randn(2 * P, device=dev, generator=g)).float()
+    x = torch.where((w.view(-1) == 0)[:, None], torch.full_like(x, float("nan")), x)
+    xr = torch.nan_to_num(x)
+    for smooth, it in ((0.0, 1.0), (0.2, 0.5)):
+        want = pair_ref(xr, t, w, ref, 0.3, smooth, it)
+        d = torch.full_like(x, float("nan"))
+        loss, margin, seq = ops.preference_loss(x, t, w, ref, beta=0.3, label_smoothing=smooth, inv_tau=it, dlogits=d)
+        close(seq, want["S"], want["dS"], "seq_logp")
+        close(margin, want["m"], want["dm"], "margin")
+        assert abs(float(loss) - float(want["loss"])) <= want["dl"] + 2 * U * abs(float(want["loss"])), "loss"
+        check_dlogits(d, want["d"], want["tol"], "dlogits")
+        l2, m2, s2 = ops.preference_loss(x, t, w, ref, beta=0.3, label_smoothing=smooth, inv_tau=it)
+        assert torch.equal(l2, loss) and torch.equal(m2, margin) and torch.equal(s2, seq)
+        xi = x.clone()
+        ops.preference_loss(xi, t, w, ref, beta=0.3, label_smoothing=smooth, inv_tau=it, dlogits=xi)
+        assert torch.equal(xi, d)
+
+
+def test_preference_loss_far_margins(dev):
+    """Margins of +-1000: the loss is the margin or zero, nothing overflows."""
+    x, t, _ = make_rows(4, 20, F32, 3, dev)
+    w = torch.ones(4, 1, device=dev)
+    ref = torch.tensor([-1000.0, 1000.0, 1000.0, -1000.0], device=dev)
+    d = torch.empty_like(x)
+    loss, margin, _ = ops.preference_loss(x, t, w, ref, beta=1.0, dlogits=d)
+    assert 1900 < float(margin[0]) < 2100 and -2100 < float(margin[1]) < -1900
+    assert abs(float(loss) + float(margin[1]) / 2) <= 1e-3
+    assert not d[0].any() and not d[2].any() and torch.isfinite(d).all() and d[1].any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_loss_modules(dev, dtype):
+    """The differentiable forms: the gradient times the upstream one, and (fp32) against differences."""
+    M, V = 12, 301
+    x, t, A, w, old, ref = make_policy(M, V, dtype, 8, dev)
+    kw = dict(old_logp=old, ref_logp=ref, kl_coef=0.1)
+    d = torch.empty_like(x)
+    loss0, logp0 = ops.policy_loss(x, t, A, w, dlogits=d, **kw)
+    xr = x.clone().requires_grad_()
+    loss, logp = hnn.policy_loss(xr, t, A, w, **kw)
+    assert loss.dim() == 0 and torch.equal(loss.detach(), loss0[0]) and torch.equal(logp, logp0) and not logp.requires_grad
+    (2.0 * loss).backward()
+    want = policy_ref(x, t, A, w, old, ref, 0.2, 0.2, 0.1, 1.0)
+    check_dlogits(xr.grad, 2 * want["d"], 2 * want["d_tol"], "policy dlogits")
+    pw = w.view(4, 3)
+    sref = torch.randn(4, device=dev, generator=gen(1)) * 3 - 20
+    ploss, margin, seq = hnn.preference_loss(xr, t, pw, sref, beta=0.2)
+    xr.grad = None
+    ploss.backward()
+    pwant = pair_ref(x, t, pw, sref, 0.2, 0.0, 1.0)
+    check_dlogits(xr.grad, pwant["d"], pwant["tol"], "preference dlogits")
+    if dtype != F32:
+        return
+    h = 2.0 ** -7
+    v = torch.randn(M, V, device=dev, generator=gen(2))
+    v = v / v.norm()
+    slope = lambda f: float(f(x + h * v).double() - f(x - h * v).double()) / (2 * h)  # noqa: E731
+    for f, grad in ((lambda z: ops.preference_loss(z, t, pw, sref, beta=0.2)[0], xr.grad),
+                    (lambda z: ops.policy_loss(z, t, A, w, clip=(0.9, 9.0), **kw)[0], None)):
+        if grad is None:  # (bounds that no ratio reaches: smooth)
+            grad = torch.empty_like(x)
+            ops.policy_loss(x, t, A, w, clip=(0.9, 9.0), dlogits=grad, **kw)
+        # |v| = 1: third derivatives are of the order of the weights' sum; rounding 256 u sum(w |lp|) / h
+        assert abs(slope(f) - float((grad.double() * v.double()).sum())) <= 30 * float(w.sum()) * (h * h + 64 * U / h)
+
+
+def test_long_offsets(dev):
+    """More than 2^31 elements of logits: the last rows are read and written where they are."""
+    V, M = 50000, 43100
+    x = torch.zeros(M, V, device=dev, dtype=BF16)
+    tail, t, A, _, old, ref = make_policy(3, V, BF16, 4, dev)
+    x[-3:] = tail
+    target = torch.zeros(M, dtype=torch.int64, device=dev)
+    target[-3:] = t
+    w, adv = torch.zeros(M, device=dev), torch.zeros(M, device=dev)
+    w[-3:], adv[-3:] = 1.0, A
+    d = torch.full_like(x, 5.0)
+    loss, logp = ops.policy_loss(x, target, adv, w, dlogits=d)
+    d0 = torch.empty_like(tail)
+    loss0, logp0 = ops.policy_loss(tail, t, A, torch.ones(3, device=dev), dlogits=d0)
+    assert torch.equal(loss, loss0) and torch.equal(logp[-3:], logp0) and torch.equal(d[-3:], d0)
+    assert not d[:-3].any()
+    _, stats = ops.token_logp(x, target, w)
+    coef = torch.zeros(M, device=dev)
+    coef[-3:] = 1
+    d.fill_(5.0)
+    ops.token_logp_bwd(x, target, stats, coef, weight=w, dlogits=d)
+    assert torch.equal(d[-3:], ops.token_logp_bwd(tail, t, stats[-3:].contiguous(), coef[-3:].contiguous()))
+    assert not d[:-3].any()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# gradient norm and clipping
+# ---------------------------------------------------------------------------------------------------------------------
+def grads_of(sizes, dev, seed=0, mixed=True):
+    g = gen(seed)
+    return [torch.randn(*s, device=dev, generator=g).to(BF16 if mixed and i % 3 == 1 else F32)
+            for i, s in enumerate(sizes)]
+
+
+def norm64(grads, kind=2.0):
+    v = torch.cat([t.reshape(-1).double() for t in grads])
+    return float(v.norm()) if kind == 2.0 else float(v.abs().max())
+
+
+SHAPES = [(7,), (300, 12), (1,), (825, 33), (4096,), (4097,), (0,), (3, 5, 7), (100000,), (64, 64), (513, 257)]
+
+
+def check_clipped(got, grads, norm, want_norm, max_norm, scale=1.0):
+    assert abs(float(norm) - want_norm) <= 2 * U * want_norm
+    f = scale * min(1.0, max_norm / (want_norm + 1e-6))
+    for o, g in zip(got, grads):
+        w = g.double() * f
+        close(o, w, w.abs() * (half(g) + 4 * U) + (2.0 ** -133 if g.dtype == BF16 else 2.0 ** -149), "clipped")
+
+
+@pytest.mark.parametrize("kind", [2.0, float("inf")])
+@pytest.mark.parametrize("max_norm", [0.0, 0.5, 1e6, float("inf")])
+def test_clip(dev, kind, max_norm):
+    grads = grads_of(SHAPES, dev)
+    keep = [g.clone() for g in grads]
+    want = norm64(grads, kind)
+    assert abs(float(ops.grad_norm(grads, kind)) - want) <= 2 * U * want
+    out = [torch.full_like(g, 9.0) for g in grads]
+    check_clipped(out, keep, ops.clip_grad_norm(grads, max_norm, kind, out=out), want, max_norm)
+    assert all(torch.equal(a, b) for a, b in zip(grads, keep))
+    norm = ops.clip_grad_norm(grads, max_norm, kind)
+    check_clipped(grads, keep, norm, want, max_norm)
+    assert all(torch.equal(a, b) for a, b in zip(grads, out))
+    assert max_norm < 1 or all(torch.equal(a, b) for a, b in zip(grads, keep))
+
+
+@pytest.mark.parametrize("count", [1, 71, 72, 73, 150, 300])
+def test_clip_many_tensors(dev, count):
+    grads = grads_of([((i * 37) % 900 + 1,) if i % 2 else (i % 7 + 1, (i * 13) % 300 + 1) for i in range(count)], dev, count)
+    keep = [g.clone() for g in grads]
+    norm = ops.clip_grad_norm(grads, 1.5, grad_scale=0.25)
+    want = 0.25 * norm64(keep)
+    check_clipped(grads, keep, norm, want, 1.5, 0.25)
+    assert torch.equal(ops.grad_norm(keep, grad_scale=-0.25), norm)
+
+
+def test_clip_layouts(dev):
+    """Padded matrix views, permuted pieces, odd starts; what lies between the rows stays as it is."""
+    g = gen(2)
+    buf = torch.randn(40000, device=dev, generator=g)
+    b16 = torch.randn(40000, device=dev, generator=g).to(BF16)
+    views = [buf[1:1 + 20 * 828].view(20, 828)[:, :825], buf[17000:17000 + 12].view(3, 4).t(),
+             buf[18001:18001 + 30 * 31].view(30, 31)[:, 1:30], buf[20001:20008],
+             b16[3:3 + 50 * 130].view(50, 130)[:, :129], b16[7001:7001 + 60].view(5, 4, 3).permute(2, 0, 1)]
+    keep, bkeep, gk = buf.clone(), b16.clone(), [v.clone() for v in views]
+    want = norm64(views)
+    norm = ops.clip_grad_norm(views, 3.0)
+    check_clipped(views, gk, norm, want, 3.0)
+    for v, k in ((buf, keep), (b16, bkeep)):
+        for a in [q for q in views if q.dtype == v.dtype]:
+            off = (a.data_ptr() - v.data_ptr()) // v.element_size()
+            a.copy_(k.as_strided(a.shape, a.stride(), off))
+        assert torch.equal(v, k), "written outside the views"
+    out = [torch.empty(20, 900, device=dev)[:, :825], torch.empty(4, 3, device=dev).t().contiguous().t()]
+    got = ops.clip_grad_norm([views[0], torch.randn(4, 3, device=dev).t().contiguous().t()], 1.0, out=out)
+    assert torch.isfinite(got).all()
+
+
+def test_norm_of_extreme_values(dev):
+    """Squares that fp32 cannot hold, and squares that vanish in it: the sum is formed in 64 bits."""
+    big, small = torch.full((1000,), 1e30, device=dev), torch.full((1000,), 1e-30, device=dev)
+    for t, v in ((big, 1e30), (small, 1e-30)):
+        want = math.sqrt(1000) * float(torch.tensor(v, dtype=F32))
+        assert abs(float(ops.grad_norm([t])) - want) <= 2 * U * want
+    ops.clip_grad_norm([big], 1.0)
+    assert abs(float(big.double().norm()) - 1.0) <= 1e-6
+    for bad in (float("nan"), float("inf")):
+        t = torch.ones(5000, device=dev)
+        t[4321] = bad
+        n, m = ops.grad_norm([t]), ops.grad_norm([t], float("inf"))
+        assert (n.isnan() and m.isnan()) if bad != bad else (n.isinf() and m.isinf())
+        u = torch.ones(3, device=dev)
+        ops.clip_grad_norm([t, u], 1.0)
+        ref = torch.ones(3) * torch.clamp(torch.tensor(1.0) / (torch.tensor(bad) + 1e-6), max=1.0)
+        assert torch.equal(u.cpu().nan_to_num(7.0), ref.nan_to_num(7.0))
+        assert t[4321].isnan()
+    assert float(ops.grad_norm([torch.zeros(10, device=dev)])) == 0.0
+    assert float(ops.grad_norm([torch.zeros(0, device=dev)])) == 0.0
+    assert float(ops.clip_grad_norm([torch.zeros(0, device=dev)], 1.0)) == 0.0
+
+
+def test_clip_parameters(dev):
+    """nn.clip_grad_norm_ on modules, beside torch's own on copies of the same gradients."""
+    lin = hnn.Linear(33, 20).to(dev)
+    ln = hnn.LayerNorm(33).to(dev)
+    unused = torch.nn.Parameter(torch.zeros(3, device=dev))
+    y = lin(ln(torch.randn(9, 33, device=dev, generator=gen(1))))
+    (y * y).sum().backward()
+    params = list(lin.parameters()) + [unused] + list(ln.parameters())
+    twin = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    for p, q in zip(params, twin):
+        q.grad = None if p.grad is None else p.grad.clone()
+    n0 = torch.nn.utils.clip_grad_norm_(twin, 0.7)
+    n1 = hnn.clip_grad_norm_(params, 0.7)
+    assert abs(float(n0) - float(n1)) <= 64 * U * float(n0)
+    for p, q in zip(params, twin):
+        assert (p.grad is None) == (q.grad is None)
+        if p.grad is not None:
+            close(p.grad, q.grad, 64 * U * q.grad.double().abs(), "clipped")
+    assert float(hnn.clip_grad_norm_([unused], 1.0)) == 0.0
+
+
+@pytest.mark.parametrize("n", [1, 5, 4099, 300001])
+def test_adam_clipped(dev, n):
+    g = gen(n)
+    mk = lambda s=1.0: s * torch.randn(n, device=dev, generator=g)  # noqa: E731
+    p, grad, m, v = mk(), mk(), mk(0.1), mk().square()
+    want = norm64([grad]) * 0.5
+    for max_norm in (0.3, 1e9):
+        a, b = [[t.clone() for t in (p, m, v)] for _ in range(2)]
+        norm = ops.adam(a[0], grad, a[1], a[2], 1e-2, 7, grad_scale=0.5, max_norm=max_norm)
+        assert abs(float(norm) - want) <= 2 * U * want
+        c = min(1.0, max_norm / (want + 1e-6))
+        ops.adam(b[0], grad, b[1], b[2], 1e-2, 7, grad_scale=0.5 * c)
+        for x, y, s in zip(a, b, (p, m, v)):  # (the two scales differ by a rounding; the update is at most a few lr)
+            close(x, y, 16 * U * (y.double().abs() + s.double().abs() + 1e-2), "adam")
+        if c == 1.0:
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+    assert ops.adam(p, grad, m, v, 1e-2, 7) is None
+
+
+def test_arena_step_is_clipped(dev):
+    """AdamState.apply(max_norm=...): padded views and fused groups; the padding adds nothing to the norm."""
+    torch.manual_seed(0)
+    named = [("a", torch.nn.Parameter(torch.randn(70, 825))), ("b", torch.nn.Parameter(torch.randn(11))),
+             ("c", torch.nn.Parameter(torch.randn(66, 70)))]
+    arenas = [ParamArena([(n, torch.nn.Parameter(p.detach().clone().to(dev))) for n, p in named], dev) for _ in range(2)]
+    g = [torch.randn(p.shape, device=dev, generator=gen(4)) for _, p in named]
+    for a in arenas:
+        for (n, _), t in zip(named, g):
+            a.grads[n].copy_(t)
+    want = norm64(g)
+    norm = arenas[0].new_adam().apply(1e-3, max_norm=want / 8)
+    assert abs(float(norm) - want) <= 2 * U * want
+    ops.clip_grad_norm(list(arenas[1].grads.values()), want / 8)
+    arenas[1].new_adam().apply(1e-3)
+    close(arenas[0].p, arenas[1].p, 1e-3 * 64 * U + 4 * U * arenas[1].p.double().abs(), "p")
+    st = arenas[0].new_adam()
+    st.sync_device_step()
+    assert abs(float(st.apply(1e-3, dynamic=True, max_norm=1.0)) - want) <= 2 * U * want
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# together, on streams, in graphs
+# ---------------------------------------------------------------------------------------------------------------------
+def tune_step(ln, fc, h, t, A, w, old):
+    """Hidden states -> layer norm -> vocabulary projection -> policy loss -> gradients -> clipping."""
+    params = list(ln.parameters()) + list(fc.parameters())
+    for p in params:
+        p.grad = None
+    logits = fc(ln(h))
+    loss, _ = hnn.policy_loss(logits, t, A, w, old_logp=old)
+    loss.backward()
+    norm = hnn.clip_grad_norm_(params, 0.05)
+    return loss.detach(), norm, [p.grad for p in params]
+
+
+def test_chain(dev):
+    """The operators as a tuning step uses them, against the same chain in 64-bit torch on the CPU."""
+    torch.manual_seed(1)
+    M, H, V = 42, 60, 500
+    ln, fc = hnn.LayerNorm(H).to(dev), hnn.Linear(H, V).to(dev)
+    h = torch.randn(M, H, device=dev, generator=gen(1)).requires_grad_()
+    t = torch.randint(0, V, (M,), device=dev, generator=gen(2))
+    A = torch.randn(M, device=dev, generator=gen(3))
+    w = (torch.rand(M, device=dev, generator=gen(4)) < 0.7).float() / M
+    ref = [torch.nn.Parameter(p.detach().double().cpu()) for p in (ln.weight, ln.bias, fc.weight, fc.bias)]
+    hr = h.detach().double().cpu().requires_grad_()
+    z = torch.nn.functional.layer_norm(hr, (H,), ref[0], ref[1]) @ ref[2].t() + ref[3]
+    lp = torch.log_softmax(z, 1).gather(1, t.cpu()[:, None])[:, 0]
+    old = (lp.detach() - 0.02 * torch.randn(M, generator=torch.Generator().manual_seed(5))).float()
+    rho = (lp - old.double()).exp()
+    Ad, wd = A.double().cpu(), w.double().cpu()
+    loss = -(wd * torch.minimum(rho * Ad, rho.clamp(0.8, 1.2) * Ad)).sum()
+    loss.backward()
+    norm = torch.nn.utils.clip_grad_norm_(ref, 0.05)
+    got_loss, got_norm, grads = tune_step(ln, fc, h, t, A, w, old.to(dev))
+    # fp32 products of H = 60 and M = 42 terms behind the operators' own roundings
+    assert abs(float(got_loss) - float(loss)) <= 1e-6 and abs(float(got_norm) - float(norm)) <= 1e-5 * float(norm)
+    for g, r in zip(grads + [h.grad], [p.grad for p in ref] + [hr.grad]):
+        assert (g.double().cpu() - r).norm() <= 1e-5 * r.norm()
+
+
+def test_other_streams(dev):
+    """Every operator on a side stream, two at once, against the default stream's answers."""
+    M, V = 64, 5000
+    jobs = []
+    for k in range(2):
+        x, t, A, w, old, ref = make_policy(M, V, BF16 if k else F32, 70 + k, dev)
+        h = torch.randn(500, 300, device=dev, generator=gen(k)).to(x.dtype)
+        jobs.append((x, t, A, w, old, ref, h))
+
+    def work(x, t, A, w, old, ref, h):
+        d = torch.empty_like(x)
+        loss, logp = ops.policy_loss(x, t, A, w, old_logp=old, ref_logp=ref, kl_coef=0.1, dlogits=d)
+        pl, pm, ps = ops.preference_loss(x, t, w.view(8, 8), torch.zeros(8, device=dev), beta=0.1)
+        y, mean, rstd = ops.layer_norm_fwd(h)
+        dx, _, db = ops.layer_norm_bwd(h, h, None, mean, rstd)
+        out = [torch.empty_like(d), torch.empty_like(dx)]
+        n = ops.clip_grad_norm([d, dx], 0.5, out=out)
+        return [loss, logp, d, pl, pm, ps, y, dx, db, n] + out
+
+    want = [work(*j) for j in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for _ in range(3):
+        got = []
+        for s, j in zip(streams, jobs):
+            with torch.cuda.stream(s):
+                got.append(work(*j))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_captured(dev):
+    """The whole chain of kernels in one graph, replayed on changing inputs with eager work in between; two graphs captured
+    on one stream and replayed at once on two do not share scratch memory."""
+    M, V, H = 48, 3001, 300
+
+    def fresh(seed):
+        x, t, A, w, old, ref = make_policy(M, V, F32, seed, dev)
+        return [x, t, A, w, old, ref, torch.randn(M, H, device=dev, generator=gen(seed))]
+
+    def work(x, t, A, w, old, ref, h):
+        d = torch.empty_like(x)
+        loss, logp = ops.policy_loss(x, t, A, w, old_logp=old, ref_logp=ref, kl_coef=0.1, dlogits=d)
+        d2 = torch.empty_like(x)
+        pl, pm, ps = ops.preference_loss(x, t, w.view(6, 8), logp[:6].contiguous(), beta=0.1, dlogits=d2)
+        y, mean, rstd = ops.layer_norm_fwd(h)
+        dx, _, db = ops.layer_norm_bwd(y, h, None, mean, rstd)
+        n = ops.clip_grad_norm([d, d2, dx], 0.5)
+        return [loss, logp, d, d2, pl, pm, ps, y, dx, db, n]
+
+    side = torch.cuda.Stream()
+    sets = []
+    with torch.cuda.stream(side):
+        work(*fresh(1))
+        torch.cuda.synchronize()
+        for k in range(2):
+            ins = fresh(10 + k)
+            graph = torch.cuda.CUDAGraph()
+            with ops.capture_without_gc():
+                with torch.cuda.graph(graph, stream=side):
+                    outs = work(*ins)
+            sets.append((graph, ins, outs))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for rep in range(4):
+        news = [fresh(100 + 10 * rep + k) for k in range(2)]
+        wants = [work(*n) for n in news]
+        for (graph, ins, _), n in zip(sets, news):
+            for a, b in zip(ins, n):
+                a.copy_(b)
+        torch.cuda.synchronize()
+        for s, (graph, _, _) in zip(streams, sets):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for (_, _, outs), want in zip(sets, wants):
+            assert all(torch.equal(p, q) for p, q in zip(outs, want)), rep
