@@ -617,7 +617,7 @@ int cgn_layer_norm_fwd(void* stream, const void* x, int64_t ldx, int64_t R, int3
                        const float* bias, float eps, void* y, int64_t ldy, float* mean, float* rstd);
 /* Its backward pass, from the statistics of the forward pass: dx (nullable; may be dy's or x's own buffer) and
  * dweight / dbias = beta * itself + the sums over the rows (nullable; R == 0 gives sums of zero).
- * workspace (with dweight or dbias): min(R, 512) * 2 * C * 4 bytes. */
+ * workspace (with dweight or dbias): min(R, 1024) * 2 * C * 4 bytes. */
 int cgn_layer_norm_bwd(void* stream, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t R, int32_t C,
                        int32_t bf16, const float* weight, const float* mean, const float* rstd, void* dx, int64_t lddx,
                        float* dweight, float* dbias, float beta, float* workspace, int64_t workspace_bytes);
@@ -673,14 +673,15 @@ typedef struct cgn_grad_tensor {
     int64_t bf16;
 } cgn_grad_tensor;
 
-/* Bytes of workspace that the two calls below need for this list (host call; 8-byte aligned). */
-int cgn_grad_norm_workspace(const cgn_grad_tensor* t, int32_t n, int64_t* bytes);
+/* Bytes of workspace that the two calls below need for this list (host call; 8-byte aligned). clip != 0: the list is
+ * for cgn_clip_grads, and refused as that refuses it. */
+int cgn_grad_norm_workspace(const cgn_grad_tensor* t, int32_t n, int32_t clip, int64_t* bytes);
 /* norm[0] = |scale| * sqrt(sum g^2) over all tensors (max_abs != 0: |scale| * max |g|); coef (nullable)
  * [0] = min(1, max_norm / (norm + 1e-6)). NaN gradients give NaN (csrc/gradnorm.hip). */
 int cgn_grad_norm(void* stream, const cgn_grad_tensor* t, int32_t n, int32_t max_abs, double scale, double max_norm,
                   float* norm, float* coef, void* workspace, int64_t workspace_bytes);
-/* The same norm, and out = g * scale * min(1, max_norm / (norm + 1e-6)) for every tensor (out may be g). Tensors must not
- * overlap each other. */
+/* The same norm, and out = g * scale * min(1, max_norm / (norm + 1e-6)) for every tensor. out may be g; apart from that
+ * no two ranges of memory (first to last element) of the list may overlap: CGN_ERR_INVALID_ARG. */
 int cgn_clip_grads(void* stream, const cgn_grad_tensor* t, int32_t n, int32_t max_abs, double scale, double max_norm,
                    float* norm, void* workspace, int64_t workspace_bytes);
 /* cgn_adam_f32 with the gradients read as g * grad_scale * clip_coef[0] (device): the update behind cgn_grad_norm. */

@@ -4,13 +4,16 @@
 // vector unit does that at its fp32 rate, far above what the loads deliver): no gradient that fp32 or bf16 holds overflows
 // or vanishes in its square, and the sum of 10^8 terms keeps its last bits. Every workgroup leaves one partial; the
 // partials are joined in a fixed order.
+#include <algorithm>
+#include <new>
+
 #include "rows.h"
 
 namespace {
 
 using namespace cgn_rows;
 
-constexpr int GN_NT = 256;
+constexpr int GN_NT = 512;
 constexpr int GN_MAX = 72;         // tensors per launch: their descriptions travel as kernel arguments (below 4 KB)
 constexpr int GN_BLOCKS = 1024;    // partials of a long list of elements: four workgroups per CU
 constexpr int64_t GN_CHUNK = 4096;  // elements a workgroup takes at least
@@ -26,6 +29,7 @@ struct Segs {
     Seg seg[GN_MAX];
     int first[GN_MAX + 1];  // first workgroup of every tensor
     int n;
+    bool stream;  // the list is past the caches' size (rows.h)
     long chunk;
 };
 
@@ -157,7 +161,7 @@ __global__ __launch_bounds__(GN_NT) void norm_final_kernel(const double* __restr
 }
 
 template <typename T>
-__device__ __forceinline__ void scale_part(const Seg& s, const Span& p, float f) {
+__device__ __forceinline__ void scale_part(const Seg& s, const Span& p, float f, bool stream) {
     constexpr int E = Piece<T>::E, U = 4;
     for (int r = p.r0; r < p.r1; ++r) {
         const T* g = (const T*)s.g + (long)r * s.ld + p.c0;
@@ -174,7 +178,10 @@ __device__ __forceinline__ void scale_part(const Seg& s, const Span& p, float f)
                     float o[E];
 #pragma unroll
                     for (int e = 0; e < E; ++e) o[e] = q[u].get(e) * f;
-                    Piece<T>::store(out + (i0 + u * GN_NT) * E, o);
+                    if (stream)
+                        Piece<T>::store_stream(out + (i0 + u * GN_NT) * E, o);
+                    else
+                        Piece<T>::store(out + (i0 + u * GN_NT) * E, o);
                 }
         }
         if (threadIdx.x < n - nfull * E)
@@ -197,9 +204,9 @@ __global__ __launch_bounds__(GN_NT) void clip_kernel(const Segs a, const double*
     const float f = (float)(scale * (double)c);
     if (f == 1.f && s.out == s.g) return;  // in place and inside the bound: nothing changes
     if (s.bf16)
-        scale_part<Bf16>(s, p, f);
+        scale_part<Bf16>(s, p, f, a.stream);
     else
-        scale_part<float>(s, p, f);
+        scale_part<float>(s, p, f, a.stream);
 }
 
 bool segs_ok(const cgn_grad_tensor* t, int n, bool out) {
@@ -212,6 +219,31 @@ bool segs_ok(const cgn_grad_tensor* t, int n, bool out) {
         if ((uintptr_t)t[i].g % al || (out && (uintptr_t)t[i].out % al)) return false;
     }
     return true;
+}
+
+// Whether no destination shares memory with another destination or with another tensor's gradient (a destination may be
+// its own gradient).
+bool apart(const cgn_grad_tensor* t, int n) {
+    struct Range {
+        uintptr_t a, b;
+        bool operator<(const Range& o) const { return a < o.a; }
+    };
+    Range* r = new (std::nothrow) Range[2 * (size_t)n + 1];
+    if (!r) return false;
+    int m = 0;
+    for (int i = 0; i < n; ++i) {
+        if (t[i].rows == 0 || t[i].cols == 0) continue;
+        const int64_t size = t[i].bf16 ? 2 : 4;
+        const uintptr_t o = (uintptr_t)t[i].out, g = (uintptr_t)t[i].g;
+        const int64_t lo = t[i].rows > 1 ? t[i].ldo : 0, lg = t[i].rows > 1 ? t[i].ld : 0;
+        r[m++] = Range{o, o + (uintptr_t)(((t[i].rows - 1) * lo + t[i].cols) * size)};
+        if (g != o || lo != lg) r[m++] = Range{g, g + (uintptr_t)(((t[i].rows - 1) * lg + t[i].cols) * size)};
+    }
+    std::sort(r, r + m);
+    bool ok = true;
+    for (int i = 1; i < m && ok; ++i) ok = r[i - 1].b <= r[i].a;
+    delete[] r;
+    return ok;
 }
 
 int64_t chunk_of(const cgn_grad_tensor* t, int n) {
@@ -232,6 +264,7 @@ int64_t blocks_of(const cgn_grad_tensor& t, int64_t chunk) {
 int pack(const cgn_grad_tensor* t, int n, int i, int64_t chunk, Segs* a, int64_t* blocks) {
     a->n = 0;
     a->chunk = chunk;
+    a->stream = chunk * GN_BLOCKS * 4 >= STREAM_BYTES;
     *blocks = 0;
     for (; i < n && a->n < GN_MAX; ++i) {
         const int64_t b = blocks_of(t[i], chunk);
@@ -300,8 +333,8 @@ int run_clip(hipStream_t s, const cgn_grad_tensor* t, int n, double scale, doubl
 
 }  // namespace
 
-extern "C" int cgn_grad_norm_workspace(const cgn_grad_tensor* t, int32_t n, int64_t* bytes) {
-    CGN_CHECK_ARG(n >= 0 && bytes && (n == 0 || t) && segs_ok(t, n, false));
+extern "C" int cgn_grad_norm_workspace(const cgn_grad_tensor* t, int32_t n, int32_t clip, int64_t* bytes) {
+    CGN_CHECK_ARG(n >= 0 && bytes && (n == 0 || t) && segs_ok(t, n, clip != 0) && (!clip || apart(t, n)));
     const int64_t parts = parts_of(t, n);
     CGN_CHECK_ARG(parts <= 0x7fffffff);
     *bytes = parts * 8 + 8;
@@ -311,7 +344,7 @@ extern "C" int cgn_grad_norm_workspace(const cgn_grad_tensor* t, int32_t n, int6
 extern "C" int cgn_grad_norm(void* stream, const cgn_grad_tensor* t, int32_t n, int32_t max_abs, double scale,
                              double max_norm, float* norm, float* coef, void* workspace, int64_t workspace_bytes) {
     int64_t need;
-    const int rc = cgn_grad_norm_workspace(t, n, &need);
+    const int rc = cgn_grad_norm_workspace(t, n, 0, &need);
     if (rc != CGN_OK) return rc;
     CGN_CHECK_ARG(norm && max_norm >= 0.0 && workspace && (uintptr_t)workspace % 8 == 0);
     if (need > workspace_bytes) return CGN_ERR_WORKSPACE;
@@ -325,9 +358,9 @@ extern "C" int cgn_grad_norm(void* stream, const cgn_grad_tensor* t, int32_t n, 
 extern "C" int cgn_clip_grads(void* stream, const cgn_grad_tensor* t, int32_t n, int32_t max_abs, double scale,
                               double max_norm, float* norm, void* workspace, int64_t workspace_bytes) {
     int64_t need;
-    const int rc = cgn_grad_norm_workspace(t, n, &need);
+    const int rc = cgn_grad_norm_workspace(t, n, 1, &need);
     if (rc != CGN_OK) return rc;
-    CGN_CHECK_ARG(segs_ok(t, n, true) && norm && max_norm >= 0.0 && workspace && (uintptr_t)workspace % 8 == 0);
+    CGN_CHECK_ARG(norm && max_norm >= 0.0 && workspace && (uintptr_t)workspace % 8 == 0);
     if (need > workspace_bytes) return CGN_ERR_WORKSPACE;
     const int parts = (int)((need - 8) / 8);
     hipStream_t s = (hipStream_t)stream;

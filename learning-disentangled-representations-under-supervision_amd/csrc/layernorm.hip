@@ -37,15 +37,18 @@ template <typename T, int NV, int G>
 struct Row {
     Piece<T> q[NV];
     float t;
-    __device__ __forceinline__ void load(const T* row, int lane, int nfull, int rem) {
+    __device__ __forceinline__ void load(const T* row, int lane, int nfull, int rem, bool stream) {
         constexpr int E = Piece<T>::E;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int i = lane + j * G;
-            if (i < nfull)
-                q[j].load(row + (long)i * E);
-            else
-                q[j].fill(0.f);
+        for (int j = 0; j < NV; ++j) q[j].fill(0.f);
+        if (stream) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                if (lane + j * G < nfull) q[j].load_stream(row + (long)(lane + j * G) * E);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                if (lane + j * G < nfull) q[j].load(row + (long)(lane + j * G) * E);
         }
         t = lane < rem ? Piece<T>::one(row + nfull * E + lane) : 0.f;
     }
@@ -81,7 +84,7 @@ template <typename T, int NT, int G, int NV>
 __global__ __launch_bounds__(NT) void layer_norm_fwd_kernel(const T* x, long ldx, long R, int C,
                                                             const float* __restrict__ w, const float* __restrict__ b,
                                                             float eps, T* y, long ldy, float* __restrict__ mean,
-                                                            float* __restrict__ rstd) {
+                                                            float* __restrict__ rstd, bool stream) {
     constexpr int E = Piece<T>::E;
     __shared__ float red[NT / 64 * 2];
     const int lane = threadIdx.x % G;
@@ -92,7 +95,7 @@ __global__ __launch_bounds__(NT) void layer_norm_fwd_kernel(const T* x, long ldx
     pb.load(b, 0.f, lane, nfull, rem);
     for (long r = (long)blockIdx.x * (NT / G) + threadIdx.x / G; r < R; r += (long)gridDim.x * (NT / G)) {
         Row<T, NV, G> row;
-        row.load(x + r * ldx, lane, nfull, rem);
+        row.load(x + r * ldx, lane, nfull, rem, stream);
         float s1[1] = {row.t};
 #pragma unroll
         for (int j = 0; j < NV; ++j)
@@ -132,7 +135,10 @@ __global__ __launch_bounds__(NT) void layer_norm_fwd_kernel(const T* x, long ldx
                 float o[E];
 #pragma unroll
                 for (int e = 0; e < E; ++e) o[e] = ((row.q[j].get(e) - mu) - off) * rs * pw.v[j][e] + pb.v[j][e];
-                Piece<T>::store(yr + (long)i * E, o);
+                if (stream)
+                    Piece<T>::store_stream(yr + (long)i * E, o);
+                else
+                    Piece<T>::store(yr + (long)i * E, o);
             }
         }
         if (lane < rem) Piece<T>::put(yr + nfull * E + lane, ((row.t - mu) - off) * rs * pw.t + pb.t);
@@ -146,7 +152,7 @@ template <typename T, int NT, int G, int NV>
 __global__ __launch_bounds__(NT) void layer_norm_bwd_kernel(const T* dy, long lddy, const T* x, long ldx, long R, int C,
                                                             const float* __restrict__ w, const float* __restrict__ mean,
                                                             const float* __restrict__ rstd, T* dx, long lddx,
-                                                            float* __restrict__ part) {
+                                                            float* __restrict__ part, bool stream) {
     constexpr int E = Piece<T>::E;
     constexpr int GROUPS = NT / G;
     __shared__ float red[NT / 64 * 3];
@@ -160,30 +166,48 @@ __global__ __launch_bounds__(NT) void layer_norm_bwd_kernel(const T* dy, long ld
     for (int j = 0; j < NV; ++j)
 #pragma unroll
         for (int e = 0; e < E; ++e) aw[j][e] = ab[j][e] = 0.f;
-    for (long r = (long)blockIdx.x * GROUPS + grp; r < R; r += (long)gridDim.x * GROUPS) {
-        Row<T, NV, G> qx, qd;
-        qx.load(x + r * ldx, lane, nfull, rem);
-        qd.load(dy + r * lddy, lane, nfull, rem);
-        const float mu = mean[r], rs = rstd[r];
-        // sums of xh, g and g xh: the first is what the stored mean's rounding left in xh, taken out below
+    long r = (long)blockIdx.x * GROUPS + grp;
+    const long step = (long)gridDim.x * GROUPS;
+    Row<T, NV, G> nx, nd;
+    float nmu = 0.f, nrs = 0.f;
+    if (r < R) {
+        nx.load(x + r * ldx, lane, nfull, rem, stream);
+        nd.load(dy + r * lddy, lane, nfull, rem, stream);
+        nmu = mean[r], nrs = rstd[r];
+    }
+    for (; r < R; r += step) {
+        Row<T, NV, G> qx = nx, qd = nd;
+        const float mu = nmu, rs = nrs;
+        if (r + step < R) {  // in flight beside this row's sums
+            nx.load(x + (r + step) * ldx, lane, nfull, rem, stream);
+            nd.load(dy + (r + step) * lddy, lane, nfull, rem, stream);
+            nmu = mean[r + step], nrs = rstd[r + step];
+        }
+        // xh = x r - mu r up to a constant of the row, the rounding of mu and of mu r: the mean of xh, which is that
+        // constant, is summed with g and g xh and taken out below
+        const float nb = -mu * rs;
         float s[3] = {0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < NV; ++j)
             if (lane + j * G < nfull) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    const float xh = (qx.q[j].get(e) - mu) * rs, g = qd.q[j].get(e) * pw.v[j][e];
+                    const float xh = fmaf(qx.q[j].get(e), rs, nb), g = qd.q[j].get(e) * pw.v[j][e];
                     s[0] += xh;
                     s[1] += g;
                     s[2] += g * xh;
                 }
             }
-        const float xht = lane < rem ? (qx.t - mu) * rs : 0.f, gt = qd.t * pw.t;
+        const float xht = lane < rem ? fmaf(qx.t, rs, nb) : 0.f, gt = qd.t * pw.t;
         s[0] += xht;
         s[1] += gt;
         s[2] += gt * xht;
         row_sums<NT, G, 3>(s, red);
+        keep_packed<T, NV>(qx.q);
+        keep_packed<T, NV>(qd.q);
         const float off = s[0] * inv_c, mg = s[1] * inv_c, mgx = s[2] * inv_c - mg * off;
+        // dx = r g - (r mgx) (xh - off) - r mg
+        const float cx = -rs * mgx, c0 = -rs * mg;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int i = lane + j * G;
@@ -192,18 +216,21 @@ __global__ __launch_bounds__(NT) void layer_norm_bwd_kernel(const T* dy, long ld
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     const float d = qd.q[j].get(e);
-                    const float xh = (qx.q[j].get(e) - mu) * rs - off;
+                    const float xh = fmaf(qx.q[j].get(e), rs, nb) - off;
                     aw[j][e] += d * xh;
                     ab[j][e] += d;
-                    o[e] = rs * ((d * pw.v[j][e] - mg) - xh * mgx);
+                    o[e] = fmaf(d * pw.v[j][e], rs, fmaf(xh, cx, c0));
                 }
-                if (dx) Piece<T>::store(dx + r * lddx + (long)i * E, o);
+                if (dx && stream)
+                    Piece<T>::store_stream(dx + r * lddx + (long)i * E, o);
+                else if (dx)
+                    Piece<T>::store(dx + r * lddx + (long)i * E, o);
             }
         }
         if (lane < rem) {
             awt += qd.t * (xht - off);
             abt += qd.t;
-            if (dx) Piece<T>::put(dx + r * lddx + nfull * E + lane, rs * ((gt - mg) - (xht - off) * mgx));
+            if (dx) Piece<T>::put(dx + r * lddx + nfull * E + lane, fmaf(gt, rs, fmaf(xht - off, cx, c0)));
         }
     }
     if (!part) return;
@@ -271,9 +298,8 @@ __global__ __launch_bounds__(LNF_NT) void layer_norm_params_kernel(const float* 
     }
 }
 
-constexpr int LN_MAX_C = 8192;    // widest row that LN_DISPATCH's groups hold in registers
-constexpr int LN_FWD_NB = 2048;   // workgroups of a forward pass at most: what is resident at once, each with many rows
-constexpr int LN_BWD_NB = 512;    // workgroups of a backward pass at most: rows of `part` it reduces at the end
+constexpr int LN_MAX_C = 8192;    // widest row that the groups below hold in registers
+constexpr int LN_FWD_NB = 8192;   // workgroups of a forward pass at most: each with many rows behind one read of w and b
 
 template <typename T, int NT, int G, int NV>
 int launch_fwd(hipStream_t s, const void* x, int64_t ldx, int64_t R, int C, const float* w, const float* b, float eps,
@@ -281,23 +307,26 @@ int launch_fwd(hipStream_t s, const void* x, int64_t ldx, int64_t R, int C, cons
     int64_t nb = (R + NT / G - 1) / (NT / G);
     if (nb > LN_FWD_NB) nb = LN_FWD_NB;
     hipLaunchKernelGGL((layer_norm_fwd_kernel<T, NT, G, NV>), dim3((unsigned)nb), dim3(NT), 0, s, (const T*)x, (long)ldx,
-                       (long)R, C, w, b, eps, (T*)y, (long)ldy, mean, rstd);
+                       (long)R, C, w, b, eps, (T*)y, (long)ldy, mean, rstd,
+                       R * C * (int64_t)sizeof(T) >= STREAM_BYTES);
     CGN_LAUNCH_CHECK();
     return CGN_OK;
 }
 
-template <typename T, int NT, int G, int NV>
+// WAVES: waves per CU that the variant's registers leave room for; as many workgroups walk the rows, and leave a row of
+// `part` each (more would only lengthen the reduction behind them).
+template <typename T, int NT, int G, int NV, int WAVES>
 int launch_bwd(hipStream_t s, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t R, int C, const float* w,
                const float* mean, const float* rstd, void* dx, int64_t lddx, float* dw, float* db, float beta,
                float* part, int64_t part_bytes) {
     int64_t nb = (R + NT / G - 1) / (NT / G);
-    if (nb > LN_BWD_NB) nb = LN_BWD_NB;
+    if (nb > 256 * WAVES * 64 / NT) nb = 256 * WAVES * 64 / NT;
     const bool params = dw || db;
     if (params && nb * 2 * C * 4 > part_bytes) return CGN_ERR_WORKSPACE;
     if (nb > 0) {
         hipLaunchKernelGGL((layer_norm_bwd_kernel<T, NT, G, NV>), dim3((unsigned)nb), dim3(NT), 0, s, (const T*)dy,
                            (long)lddy, (const T*)x, (long)ldx, (long)R, C, w, mean, rstd, (T*)dx, (long)lddx,
-                           params ? part : nullptr);
+                           params ? part : nullptr, R * C * (int64_t)sizeof(T) >= STREAM_BYTES);
         CGN_LAUNCH_CHECK();
     }
     if (params) {
@@ -308,31 +337,60 @@ int launch_bwd(hipStream_t s, const void* dy, int64_t lddy, const void* x, int64
     return CGN_OK;
 }
 
-// The narrowest group whose lanes hold the row in at most 16 elements each (with the backward pass's sums that is what
-// stays in registers): narrow rows share a wave, wide ones take a workgroup.
-#define LN_DISPATCH(fn, ...)                                                      \
-    do {                                                                          \
-        const int n__ = cgn_cdiv(C, bf16 ? 8 : 4); /* pieces of a row */          \
-        if (bf16) {                                                               \
-            if (n__ <= 8) return fn<Bf16, 256, 8, 1>(__VA_ARGS__);                \
-            if (n__ <= 16) return fn<Bf16, 256, 16, 1>(__VA_ARGS__);              \
-            if (n__ <= 32) return fn<Bf16, 256, 32, 1>(__VA_ARGS__);              \
-            if (n__ <= 64) return fn<Bf16, 256, 64, 1>(__VA_ARGS__);              \
-            if (n__ <= 128) return fn<Bf16, 256, 64, 2>(__VA_ARGS__);             \
-            if (n__ <= 256) return fn<Bf16, 256, 256, 1>(__VA_ARGS__);            \
-            if (n__ <= 512) return fn<Bf16, 256, 256, 2>(__VA_ARGS__);            \
-            return fn<Bf16, 1024, 1024, 1>(__VA_ARGS__);                          \
-        }                                                                         \
-        if (n__ <= 8) return fn<float, 256, 8, 1>(__VA_ARGS__);                   \
-        if (n__ <= 16) return fn<float, 256, 16, 1>(__VA_ARGS__);                 \
-        if (n__ <= 32) return fn<float, 256, 32, 1>(__VA_ARGS__);                 \
-        if (n__ <= 64) return fn<float, 256, 64, 1>(__VA_ARGS__);                 \
-        if (n__ <= 128) return fn<float, 256, 64, 2>(__VA_ARGS__);                \
-        if (n__ <= 256) return fn<float, 256, 64, 4>(__VA_ARGS__);                \
-        if (n__ <= 512) return fn<float, 256, 256, 2>(__VA_ARGS__);               \
-        if (n__ <= 1024) return fn<float, 256, 256, 4>(__VA_ARGS__);              \
-        return fn<float, 1024, 1024, 2>(__VA_ARGS__);                             \
-    } while (0)
+// The narrowest group whose lanes hold the row in a few pieces: narrow rows share a wave, wide ones take a workgroup.
+template <typename T>
+int norm_fwd(hipStream_t s, const void* x, int64_t ldx, int64_t R, int C, const float* w, const float* b, float eps,
+             void* y, int64_t ldy, float* mean, float* rstd) {
+    const int n = cgn_cdiv(C, Piece<T>::E);
+#define LN_FWD(NT, G, NV) return launch_fwd<T, NT, G, NV>(s, x, ldx, R, C, w, b, eps, y, ldy, mean, rstd)
+    if (n <= 8) LN_FWD(256, 8, 1);
+    if (n <= 16) LN_FWD(256, 16, 1);
+    if (n <= 32) LN_FWD(256, 32, 1);
+    if (n <= 64) LN_FWD(256, 64, 1);
+    if (n <= 128) LN_FWD(256, 64, 2);
+    if constexpr (Piece<T>::E == 4) {
+        if (n <= 256) LN_FWD(256, 64, 4);
+    } else {
+        if (n <= 256) LN_FWD(256, 256, 1);
+    }
+    if (n <= 512) LN_FWD(256, 256, 2);
+    if constexpr (Piece<T>::E == 4) {
+        if (n <= 1024) LN_FWD(256, 256, 4);
+        LN_FWD(1024, 1024, 2);
+    } else {
+        LN_FWD(1024, 1024, 1);
+    }
+#undef LN_FWD
+}
+
+// A lane's share of a row is kept at 16 elements: row, gradient, weight, the two sums and the next row's loads fit 128 to
+// 160 registers.
+template <typename T>
+int norm_bwd(hipStream_t s, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t R, int C, const float* w,
+             const float* mean, const float* rstd, void* dx, int64_t lddx, float* dw, float* db, float beta, float* part,
+             int64_t part_bytes) {
+    const int n = cgn_cdiv(C, Piece<T>::E);
+#define LN_BWD(NT, G, NV, WAVES)                                                                                       \
+    return launch_bwd<T, NT, G, NV, WAVES>(s, dy, lddy, x, ldx, R, C, w, mean, rstd, dx, lddx, dw, db, beta, part,     \
+                                           part_bytes)
+    if (n <= 8) LN_BWD(512, 8, 1, 16);
+    if (n <= 16) LN_BWD(512, 16, 1, 16);
+    if (n <= 32) LN_BWD(512, 32, 1, 16);
+    if (n <= 64) LN_BWD(512, 64, 1, 16);
+    if constexpr (Piece<T>::E == 4) {
+        if (n <= 128) LN_BWD(512, 64, 2, 16);
+        if (n <= 256) LN_BWD(256, 64, 4, 8);
+        if (n <= 512) LN_BWD(256, 256, 2, 12);
+        if (n <= 1024) LN_BWD(512, 512, 2, 16);
+        LN_BWD(1024, 1024, 2, 16);
+    } else {
+        if (n <= 128) LN_BWD(256, 64, 2, 12);
+        if (n <= 256) LN_BWD(256, 256, 1, 12);
+        if (n <= 512) LN_BWD(512, 512, 1, 16);
+        LN_BWD(1024, 1024, 1, 16);
+    }
+#undef LN_BWD
+}
 
 }  // namespace
 
@@ -343,7 +401,8 @@ extern "C" int cgn_layer_norm_fwd(void* stream, const void* x, int64_t ldx, int6
     if (R == 0) return CGN_OK;
     CGN_CHECK_ARG(x && y && mean && rstd);
     hipStream_t s = (hipStream_t)stream;
-    LN_DISPATCH(launch_fwd, s, x, ldx, R, C, weight, bias, eps, y, ldy, mean, rstd);
+    return bf16 ? norm_fwd<Bf16>(s, x, ldx, R, C, weight, bias, eps, y, ldy, mean, rstd)
+                : norm_fwd<float>(s, x, ldx, R, C, weight, bias, eps, y, ldy, mean, rstd);
 }
 
 extern "C" int cgn_layer_norm_bwd(void* stream, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t R,
@@ -354,6 +413,8 @@ extern "C" int cgn_layer_norm_bwd(void* stream, const void* dy, int64_t lddy, co
     CGN_CHECK_ARG(R == 0 || (dy && x && mean && rstd));
     CGN_CHECK_ARG((!dweight && !dbias) || R == 0 || workspace);
     hipStream_t s = (hipStream_t)stream;
-    LN_DISPATCH(launch_bwd, s, dy, lddy, x, ldx, R, C, weight, mean, rstd, dx, lddx, dweight, dbias, beta, workspace,
-                workspace_bytes);
+    return bf16 ? norm_bwd<Bf16>(s, dy, lddy, x, ldx, R, C, weight, mean, rstd, dx, lddx, dweight, dbias, beta, workspace,
+                                 workspace_bytes)
+                : norm_bwd<float>(s, dy, lddy, x, ldx, R, C, weight, mean, rstd, dx, lddx, dweight, dbias, beta,
+                                  workspace, workspace_bytes);
 }

@@ -5,7 +5,13 @@
 #pragma once
 #include "common.h"
 
+// load_stream / store_stream mark data that will not be read again before the 256 MB cache has seen its size in other
+// data: it then neither pushes out what is wanted nor leaves dirty lines for later reads to wait on. A copy of 512 MB with
+// both marks runs at 6.3 TB/s, without them at 5.6 (5.1 to 5.2 with few, long-running workgroups).
+
 namespace cgn_rows {
+
+constexpr int64_t STREAM_BYTES = 128 << 20;  // data from this size on is streamed: half of the cache
 
 struct Bf16 {
     unsigned short bits;
@@ -32,10 +38,17 @@ struct Piece<float> {
     static constexpr int E = 4;
     f32x4 v;
     __device__ __forceinline__ void load(const float* p) { v = *reinterpret_cast<const f32x4_e4*>(p); }
+    __device__ __forceinline__ void load_stream(const float* p) {
+        v = __builtin_nontemporal_load(reinterpret_cast<const f32x4_e4*>(p));
+    }
     __device__ __forceinline__ void fill(float x) { v = f32x4{x, x, x, x}; }
     __device__ __forceinline__ float get(int e) const { return v[e]; }
     static __device__ __forceinline__ void store(float* p, const float (&o)[E]) {
         *reinterpret_cast<f32x4_e4*>(p) = f32x4{o[0], o[1], o[2], o[3]};
+    }
+    static __device__ __forceinline__ void store_stream(float* p, const float (&o)[E]) {
+        const f32x4_e4 w = {o[0], o[1], o[2], o[3]};
+        __builtin_nontemporal_store(w, reinterpret_cast<f32x4_e4*>(p));
     }
     static __device__ __forceinline__ void put(float* p, float x) { *p = x; }
     static __device__ __forceinline__ float one(const float* p) { return *p; }
@@ -46,6 +59,9 @@ struct Piece<Bf16> {
     static constexpr int E = 8;
     unsigned v __attribute__((ext_vector_type(4)));
     __device__ __forceinline__ void load(const Bf16* p) { v = *reinterpret_cast<const u32x4_e2*>(p); }
+    __device__ __forceinline__ void load_stream(const Bf16* p) {
+        v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_e2*>(p));
+    }
     __device__ __forceinline__ void fill(float x) {
         const unsigned h = f32_to_bf16(x), w = h | h << 16;
 #pragma unroll
@@ -55,16 +71,31 @@ struct Piece<Bf16> {
         const unsigned w = v[e >> 1];
         return __builtin_bit_cast(float, e & 1 ? w & 0xffff0000u : w << 16);
     }
-    static __device__ __forceinline__ void store(Bf16* p, const float (&o)[E]) {
-        unsigned w __attribute__((ext_vector_type(4)));
+    static __device__ __forceinline__ u32x4_e2 pack(const float (&o)[E]) {
+        u32x4_e2 w;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             w[e] = __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{o[2 * e], o[2 * e + 1]}, bf16x2));
-        *reinterpret_cast<u32x4_e2*>(p) = w;
+        return w;
+    }
+    static __device__ __forceinline__ void store(Bf16* p, const float (&o)[E]) { *reinterpret_cast<u32x4_e2*>(p) = pack(o); }
+    static __device__ __forceinline__ void store_stream(Bf16* p, const float (&o)[E]) {
+        __builtin_nontemporal_store(pack(o), reinterpret_cast<u32x4_e2*>(p));
     }
     static __device__ __forceinline__ void put(Bf16* p, float x) { p->bits = f32_to_bf16(x); }
     static __device__ __forceinline__ float one(const Bf16* p) { return bf16_to_f32(p->bits); }
 };
+
+// bf16 rows stay packed (two elements a register) from pass to pass over them and are unpacked, and take their
+// exponentials, anew: kept, the floats would need twice the registers and halve the waves per CU. The compiler must not
+// see that the passes form the same values. (fp32 rows are as they are.)
+template <typename T, int NV>
+__device__ __forceinline__ void keep_packed(Piece<T> (&q)[NV]) {
+    if constexpr (Piece<T>::E == 8) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) asm volatile("" : "+v"(q[j].v));
+    }
+}
 
 // Sum over the G lanes of a group (G a power of two up to the wave); every lane gets it.
 template <int G>

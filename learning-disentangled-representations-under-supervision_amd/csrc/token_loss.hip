@@ -33,41 +33,52 @@ struct RowArgs {
     float* coef;       // [M], nullable: d loss / d lp of the row
     void* dlogits;     // may be the logits' own buffer
     long ldd;
+    bool stream_in, stream_out;  // logits / dlogits are past the caches' size (rows.h)
 };
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Everything of a row that is one number; called by one thread. Returns d loss / d lp.
-template <typename T>
-__device__ __forceinline__ float row_scalars(const RowArgs& a, long row, float w, float inv_tau, float m, float z) {
-    const int64_t t = a.target[row];
-    // (an out-of-range target gives NaN, never an out-of-bounds read)
-    const bool in = t >= 0 && t < a.V;
-    const double xt = in ? (double)Piece<T>::one((const T*)a.logits + row * a.ld + t) : (double)NAN;
-    const double lp = (xt - (double)m) * (double)inv_tau - (double)logf(z);
-    if (a.logp) a.logp[row] = (float)lp;
-    if (a.lp64) a.lp64[row] = lp * (double)w;
-    if (a.stats) {
-        a.stats[2 * row] = m;
-        a.stats[2 * row + 1] = z;
+// Everything of a row that is one number. One thread loads it before the row itself and finishes it once the row's
+// maximum and total are known, so that its dependent loads (target, then the target's logit) pass beside the row's.
+struct RowScalars {
+    float xt, A, old_logp, ref_logp;
+
+    template <typename T>
+    __device__ __forceinline__ void load(const RowArgs& a, long row) {
+        const int64_t t = a.target[row];
+        A = a.advantage ? a.advantage[row] : 0.f;
+        old_logp = a.old_logp ? a.old_logp[row] : 0.f;
+        ref_logp = a.ref_logp ? a.ref_logp[row] : 0.f;
+        // (an out-of-range target gives NaN, never an out-of-bounds read)
+        xt = t >= 0 && t < a.V ? Piece<T>::one((const T*)a.logits + row * a.ld + t) : NAN;
     }
-    if (!a.advantage) return 0.f;
-    const float A = a.advantage[row];
-    const float ratio = a.old_logp ? expf((float)(lp - (double)a.old_logp[row])) : 1.f;
-    const float lim = fminf(fmaxf(ratio, 1.f - a.clip_lo), 1.f + a.clip_hi);
-    const bool cut = (A > 0.f && ratio > 1.f + a.clip_hi) || (A < 0.f && ratio < 1.f - a.clip_lo);
-    float loss = -(cut ? lim : ratio) * A, g = cut ? 0.f : -ratio * A;
-    if (a.ref_logp) {
-        // exp(k) - k - 1 and its derivative through expm1: k is small where the two policies agree
-        const float k = (float)((double)a.ref_logp[row] - lp), e = expm1f(k);
-        loss += a.kl_coef * (e - k);
-        g -= a.kl_coef * e;
+
+    // writes the row's results; returns d loss / d lp
+    __device__ __forceinline__ float finish(const RowArgs& a, long row, float w, float inv_tau, float m, float z) const {
+        const double lp = ((double)xt - (double)m) * (double)inv_tau - (double)logf(z);
+        if (a.logp) a.logp[row] = (float)lp;
+        if (a.lp64) a.lp64[row] = lp * (double)w;
+        if (a.stats) {
+            a.stats[2 * row] = m;
+            a.stats[2 * row + 1] = z;
+        }
+        if (!a.advantage) return 0.f;
+        const float ratio = a.old_logp ? expf((float)(lp - (double)old_logp)) : 1.f;
+        const float lim = fminf(fmaxf(ratio, 1.f - a.clip_lo), 1.f + a.clip_hi);
+        const bool cut = (A > 0.f && ratio > 1.f + a.clip_hi) || (A < 0.f && ratio < 1.f - a.clip_lo);
+        float loss = -(cut ? lim : ratio) * A, g = cut ? 0.f : -ratio * A;
+        if (a.ref_logp) {
+            // exp(k) - k - 1 and its derivative through expm1: k is small where the two policies agree
+            const float k = (float)((double)ref_logp - lp), e = expm1f(k);
+            loss += a.kl_coef * (e - k);
+            g -= a.kl_coef * e;
+        }
+        a.row_loss[row] = (double)loss * (double)w;
+        g *= w;
+        if (a.coef) a.coef[row] = g;
+        return g;
     }
-    a.row_loss[row] = (double)loss * (double)w;
-    g *= w;
-    if (a.coef) a.coef[row] = g;
-    return g;
-}
+};
 
 __device__ __forceinline__ void masked_scalars(const RowArgs& a, long row) {
     if (a.logp) a.logp[row] = 0.f;
@@ -80,52 +91,95 @@ __device__ __forceinline__ void masked_scalars(const RowArgs& a, long row) {
     if (a.coef) a.coef[row] = 0.f;
 }
 
-template <typename T, int NT>
-__device__ __forceinline__ void zero_row(T* d, int V) {
-    constexpr int E = Piece<T>::E;
-    const int nfull = V / E, rem = V % E;
-    float o[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.f;
-    for (int i = threadIdx.x; i < nfull; i += NT) Piece<T>::store(d + (long)i * E, o);
-    if (threadIdx.x < rem) Piece<T>::put(d + nfull * E + threadIdx.x, 0.f);
+template <typename T>
+__device__ __forceinline__ void put_piece(T* p, const float (&o)[Piece<T>::E], bool stream) {
+    if (stream)
+        Piece<T>::store_stream(p, o);
+    else
+        Piece<T>::store(p, o);
 }
 
-// One workgroup per row, the row in registers (NV 16-byte pieces per thread and one single element of the V % E last).
+// A row cut at the 128-byte lines of its buffer: `head` elements up to the first line, nfull whole 16-byte pieces from
+// there on, the rest behind them. The head's and the rest's elements (at most 70) go one to a thread. The accesses of a wave
+// are then whole lines: on rows that start 32 bytes into a line a copy of this shape loses a tenth without it.
+template <typename T>
+struct Cut {
+    static constexpr int E = Piece<T>::E;
+    int head, nfull, edge;
+    __device__ __forceinline__ Cut(const T* row, int V) {
+        head = (int)((128 - ((uintptr_t)row & 127)) & 127) / (int)sizeof(T);
+        head = head < V ? head : V;
+        nfull = (V - head) / E;
+        edge = V - nfull * E;
+    }
+    __device__ __forceinline__ long piece(int i) const { return (long)i * E + head; }
+    __device__ __forceinline__ int edge_col(int t) const { return t < head ? t : nfull * E + t; }
+};
+
+template <typename T, int NT>
+__device__ __forceinline__ void zero_row(T* d, int V, bool stream) {
+    const Cut<T> cut(d, V);
+    float o[Piece<T>::E];
+#pragma unroll
+    for (int e = 0; e < Piece<T>::E; ++e) o[e] = 0.f;
+    for (int i = threadIdx.x; i < cut.nfull; i += NT) put_piece<T>(d + cut.piece(i), o, stream);
+    if ((int)threadIdx.x < cut.edge) Piece<T>::put(d + cut.edge_col(threadIdx.x), 0.f);
+}
+
+// Pieces threadIdx.x, threadIdx.x + NT, ... of a row; what lies past its last piece reads as -inf.
+template <typename T, int NT, int NV>
+__device__ __forceinline__ void load_all(Piece<T> (&q)[NV], const T* x, const Cut<T>& cut, bool stream) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) q[j].fill(-INFINITY);
+    if (stream) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if ((int)threadIdx.x + j * NT < cut.nfull) q[j].load_stream(x + cut.piece(threadIdx.x + j * NT));
+    } else {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if ((int)threadIdx.x + j * NT < cut.nfull) q[j].load(x + cut.piece(threadIdx.x + j * NT));
+    }
+}
+
+// One workgroup per row, the row in registers: NV 16-byte pieces per thread and one single element of its ragged ends.
 template <typename T, int NT, int NV>
 __global__ __launch_bounds__(NT) void row_kernel(const RowArgs a) {
-    constexpr int E = Piece<T>::E;
-    __shared__ float red[NT / 64 + 1];
+    constexpr int E = Piece<T>::E, NW = NT / 64;
+    __shared__ float red_m[NW], red_z[NW];
     __shared__ float coef_s;
     const long row = blockIdx.x;
     const float w = a.weight ? a.weight[row] : 1.f;
     T* d = a.dlogits ? (T*)a.dlogits + row * a.ldd : nullptr;
     if (w == 0.f) {
-        if (d) zero_row<T, NT>(d, a.V);
+        if (d) zero_row<T, NT>(d, a.V, a.stream_out);
         if (threadIdx.x == 0) masked_scalars(a, row);
         return;
     }
     const float inv_tau = a.dyn_inv_tau ? a.dyn_inv_tau[0] : a.inv_tau;
     const T* x = (const T*)a.logits + row * a.ld;
-    const int nfull = a.V / E, rem = a.V % E;
+    const Cut<T> cut(x, a.V);
+    const bool has_edge = (int)threadIdx.x < cut.edge;
+    const int ec = cut.edge_col(threadIdx.x);
+    RowScalars rs;
+    if (threadIdx.x == 0) rs.load<T>(a, row);
     Piece<T> q[NV];
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int i = threadIdx.x + j * NT;
-        if (i < nfull)
-            q[j].load(x + (long)i * E);
-        else
-            q[j].fill(-INFINITY);
-    }
-    const float xt = threadIdx.x < rem ? Piece<T>::one(x + nfull * E + threadIdx.x) : -INFINITY;
-    float m = xt;
+    load_all<T, NT, NV>(q, x, cut, a.stream_in);
+    const float xe = has_edge ? Piece<T>::one(x + ec) : -INFINITY;
+    float m = xe;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
         for (int e = 0; e < E; ++e) m = fmaxf(m, q[j].get(e));
-    m = block_max<NT>(m, red);
+    m = wave_max(m);
+    if ((threadIdx.x & 63) == 0) red_m[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = red_m[0];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) m = fmaxf(m, red_m[i]);
+    keep_packed<T, NV>(q);
     const float c2 = inv_tau * LOG2E;
-    const float et = fast_exp2((xt - m) * c2);
+    const float pe = fast_exp2((xe - m) * c2);
     float part[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) part[e] = 0.f;
@@ -133,20 +187,27 @@ __global__ __launch_bounds__(NT) void row_kernel(const RowArgs a) {
     for (int j = 0; j < NV; ++j)
 #pragma unroll
         for (int e = 0; e < E; ++e) part[e] += fast_exp2((q[j].get(e) - m) * c2);
-    float z = et;
+    float z = pe;
 #pragma unroll
     for (int e = 0; e < E; ++e) z += part[e];
-    z = block_sum<NT>(z, red);
-    if (threadIdx.x == 0) coef_s = row_scalars<T>(a, row, w, inv_tau, m, z);
+    z = wave_sum(z);
+    if ((threadIdx.x & 63) == 0) red_z[threadIdx.x >> 6] = z;
+    __syncthreads();
+    z = 0.f;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) z += red_z[i];
+    if (threadIdx.x == 0) coef_s = rs.finish(a, row, w, inv_tau, m, z);
     if (!d) return;
     __syncthreads();
+    keep_packed<T, NV>(q);
     const float c = coef_s * inv_tau, cz = -c / z;
-    const int64_t t = a.target[row];
-    const int tp = t >= 0 && t < a.V ? (int)t / E : -1, te = (int)t % E;
+    const int64_t t64 = a.target[row];
+    const int t = t64 >= 0 && t64 < a.V ? (int)t64 : -1;
+    const int tp = t < cut.head ? -1 : (t - cut.head) / E, te = t - cut.head - tp * E;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int i = threadIdx.x + j * NT;
-        if (i < nfull) {
+        if (i < cut.nfull) {
             float o[E];
 #pragma unroll
             for (int e = 0; e < E; ++e) o[e] = fast_exp2((q[j].get(e) - m) * c2) * cz;
@@ -154,11 +215,10 @@ __global__ __launch_bounds__(NT) void row_kernel(const RowArgs a) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) o[e] += e == te ? c : 0.f;
             }
-            Piece<T>::store(d + (long)i * E, o);
+            put_piece<T>(d + cut.piece(i), o, a.stream_out);
         }
     }
-    if (threadIdx.x < rem)
-        Piece<T>::put(d + nfull * E + threadIdx.x, et * cz + (tp == nfull && te == (int)threadIdx.x ? c : 0.f));
+    if (has_edge) Piece<T>::put(d + ec, pe * cz + (ec == t ? c : 0.f));
 }
 
 // A row too long for the registers of a workgroup: running maximum and total per thread, joined at the end.
@@ -175,15 +235,15 @@ __global__ __launch_bounds__(NT) void row_stream_kernel(const RowArgs a) {
     const float inv_tau = a.dyn_inv_tau ? a.dyn_inv_tau[0] : a.inv_tau;
     const float c2 = inv_tau * LOG2E;
     const T* x = (const T*)a.logits + row * a.ld;
-    const int nfull = a.V / E, rem = a.V % E;
+    const Cut<T> cut(x, a.V);
     constexpr int U = 4;  // pieces in flight
     float m = -INFINITY, z = 0.f;
-    for (int i0 = threadIdx.x; i0 < nfull; i0 += U * NT) {
+    for (int i0 = threadIdx.x; i0 < cut.nfull; i0 += U * NT) {
         Piece<T> q[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (i0 + u * NT < nfull)
-                q[u].load(x + (long)(i0 + u * NT) * E);
+            if (i0 + u * NT < cut.nfull)
+                q[u].load(x + cut.piece(i0 + u * NT));
             else
                 q[u].fill(-INFINITY);
         }
@@ -203,11 +263,15 @@ __global__ __launch_bounds__(NT) void row_stream_kernel(const RowArgs a) {
             z += p;
         }
     }
-    const float xt = threadIdx.x < rem ? Piece<T>::one(x + nfull * E + threadIdx.x) : -INFINITY;
-    const float mb = block_max<NT>(fmaxf(m, xt), red);
+    const float xe = (int)threadIdx.x < cut.edge ? Piece<T>::one(x + cut.edge_col(threadIdx.x)) : -INFINITY;
+    const float mb = block_max<NT>(fmaxf(m, xe), red);
     const float mine = m == -INFINITY && z == 0.f ? 0.f : z * fast_exp2((m - mb) * c2);
-    z = block_sum<NT>(mine + fast_exp2((xt - mb) * c2), red);
-    if (threadIdx.x == 0) row_scalars<T>(a, row, w, inv_tau, mb, z);
+    z = block_sum<NT>(mine + fast_exp2((xe - mb) * c2), red);
+    if (threadIdx.x == 0) {
+        RowScalars rs;
+        rs.load<T>(a, row);
+        rs.finish(a, row, w, inv_tau, mb, z);
+    }
 }
 
 struct GradArgs {
@@ -223,34 +287,49 @@ struct GradArgs {
     const float* scale;  // nullable: one factor on the device (the gradient of the loss itself)
     void* dlogits;       // may be the logits' own buffer: every element is read and written by one thread
     long ldd;
+    bool stream_out;
+    int chunks;  // workgroups per row
 };
 
-template <typename T, int NT>
+// grid: row by row, `chunks` workgroups each, of U pieces per thread and no loop. Many short workgroups stream better than
+// few long ones: they keep the addresses in flight together.
+template <typename T, int NT, int U>
 __global__ __launch_bounds__(NT) void row_grad_kernel(const GradArgs a) {
     constexpr int E = Piece<T>::E;
-    const long row = blockIdx.x;
+    const int chunk = blockIdx.x % a.chunks;
+    const long row = gridDim.x / a.chunks - 1 - blockIdx.x / a.chunks;  // backwards: the statistics' pass has left the
+                                                                        // last rows in the cache
     T* d = (T*)a.dlogits + row * a.ldd;
+    const Cut<T> cut(d, a.V);
+    const int i0 = chunk * (NT * U) + threadIdx.x;
+    const bool has_edge = chunk == 0 && (int)threadIdx.x < cut.edge;
     if (a.weight && a.weight[row] == 0.f) {
-        zero_row<T, NT>(d, a.V);
+        float o[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i0 + u * NT < cut.nfull) put_piece<T>(d + cut.piece(i0 + u * NT), o, a.stream_out);
+        if (has_edge) Piece<T>::put(d + cut.edge_col(threadIdx.x), 0.f);
         return;
     }
+    const T* x = (const T*)a.logits + row * a.ld;
+    Piece<T> q[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (i0 + u * NT < cut.nfull) q[u].load(x + cut.piece(i0 + u * NT));
+    const int ec = cut.edge_col(threadIdx.x);
+    const float xe = has_edge ? Piece<T>::one(x + ec) : 0.f;
     const float inv_tau = a.dyn_inv_tau ? a.dyn_inv_tau[0] : a.inv_tau;
     const float c2 = inv_tau * LOG2E, m = a.stats[2 * row], z = a.stats[2 * row + 1];
     const float c = a.coef[row] * (a.scale ? a.scale[0] : 1.f) * inv_tau, cz = -c / z;
-    const T* x = (const T*)a.logits + row * a.ld;
-    const int nfull = a.V / E, rem = a.V % E;
-    const int64_t t = a.target[row];
-    const int tp = t >= 0 && t < a.V ? (int)t / E : -1, te = (int)t % E;
-    constexpr int U = 4;
-    for (int i0 = threadIdx.x; i0 < nfull; i0 += U * NT) {
-        Piece<T> q[U];
+    const int64_t t64 = a.target[row];
+    const int t = t64 >= 0 && t64 < a.V ? (int)t64 : -1;
+    const int tp = t < cut.head ? -1 : (t - cut.head) / E, te = t - cut.head - tp * E;
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (i0 + u * NT < nfull) q[u].load(x + (long)(i0 + u * NT) * E);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = i0 + u * NT;
-            if (i >= nfull) break;
+    for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * NT;
+        if (i < cut.nfull) {
             float o[E];
 #pragma unroll
             for (int e = 0; e < E; ++e) o[e] = fast_exp2((q[u].get(e) - m) * c2) * cz;
@@ -258,13 +337,10 @@ __global__ __launch_bounds__(NT) void row_grad_kernel(const GradArgs a) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) o[e] += e == te ? c : 0.f;
             }
-            Piece<T>::store(d + (long)i * E, o);
+            put_piece<T>(d + cut.piece(i), o, a.stream_out);
         }
     }
-    if (threadIdx.x < rem) {
-        const float p = fast_exp2((Piece<T>::one(x + nfull * E + threadIdx.x) - m) * c2);
-        Piece<T>::put(d + nfull * E + threadIdx.x, p * cz + (tp == nfull && te == (int)threadIdx.x ? c : 0.f));
-    }
+    if (has_edge) Piece<T>::put(d + ec, fast_exp2((xe - m) * c2) * cz + (ec == t ? c : 0.f));
 }
 
 __device__ __forceinline__ double wave_sum64(double v) {
@@ -279,12 +355,19 @@ __global__ __launch_bounds__(SUM_NT) void sum64_kernel(const double* __restrict_
                                                        float* __restrict__ out) {
     __shared__ double red[SUM_NT / 64];
     double s = 0.0;
-    for (long i = threadIdx.x; i < n; i += SUM_NT) s += v[i];
+    for (long i0 = threadIdx.x; i0 < n; i0 += 8 * SUM_NT) {
+        double q[8];  // loads in flight
+#pragma unroll
+        for (int u = 0; u < 8; ++u) q[u] = i0 + u * SUM_NT < n ? v[i0 + u * SUM_NT] : 0.0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) s += q[u];
+    }
     s = wave_sum64(s);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x == 0) {
         double t = 0.0;
+#pragma unroll
         for (int i = 0; i < SUM_NT / 64; ++i) t += red[i];
         out[0] = (float)(t * scale);
     }
@@ -332,9 +415,23 @@ int launch_row(hipStream_t s, const RowArgs& a, int64_t M) {
 }
 
 template <typename T>
-int launch_grad(hipStream_t s, const GradArgs& g, int64_t M) {
-    hipLaunchKernelGGL((row_grad_kernel<T, 512>), dim3((unsigned)M), dim3(512), 0, s, g);
-    CGN_LAUNCH_CHECK();
+int launch_grad(hipStream_t s, GradArgs g, int64_t M) {
+    constexpr int NT = 256, U = 2;
+    g.chunks = cgn_cdiv(g.V, (long)Piece<T>::E * NT * U);
+    // whole rows per launch, as many as a grid holds
+    const int64_t most = 0x7fffffff / g.chunks;
+    for (int64_t r = M; r > 0; r -= most) {
+        const int64_t n = r < most ? r : most, r0 = r - n;
+        GradArgs b = g;
+        b.logits = (const T*)g.logits + r0 * g.ld;
+        b.dlogits = (T*)g.dlogits + r0 * g.ldd;
+        b.target += r0;
+        if (b.weight) b.weight += r0;
+        b.stats += 2 * r0;
+        b.coef += r0;
+        hipLaunchKernelGGL((row_grad_kernel<T, NT, U>), dim3((unsigned)(n * g.chunks)), dim3(NT), 0, s, b);
+        CGN_LAUNCH_CHECK();
+    }
     return CGN_OK;
 }
 
@@ -344,14 +441,19 @@ template <typename T>
 int launch_rows(hipStream_t s, RowArgs a, int64_t M, bool* done) {
     const int n = cgn_cdiv(a.V, Piece<T>::E);
     *done = true;
+#ifdef VAR
+    VAR
+#endif
     if (n <= 256 * 1) return launch_row<T, 256, 1>(s, a, M);
     if (n <= 256 * 2) return launch_row<T, 256, 2>(s, a, M);
     if (n <= 256 * 4) return launch_row<T, 256, 4>(s, a, M);
-    if (n <= 256 * 8) return launch_row<T, 256, 8>(s, a, M);
-    if (n <= 512 * 8) return launch_row<T, 512, 8>(s, a, M);
-    if (n <= 512 * 12) return launch_row<T, 512, 12>(s, a, M);
-    if (n <= 512 * 16) return launch_row<T, 512, 16>(s, a, M);
-    if (n <= 1024 * 12) return launch_row<T, 1024, 12>(s, a, M);
+    if (n <= 1024 * 2) return launch_row<T, 1024, 2>(s, a, M);
+    if (n <= 1024 * 3) return launch_row<T, 1024, 3>(s, a, M);
+    if (n <= 1024 * 4) return launch_row<T, 1024, 4>(s, a, M);
+    if (n <= 1024 * 5) return launch_row<T, 1024, 5>(s, a, M);
+    if (n <= 1024 * 7) return launch_row<T, 1024, 7>(s, a, M);
+    if (n <= 1024 * 10) return launch_row<T, 1024, 10>(s, a, M);
+    if (n <= 1024 * 13) return launch_row<T, 1024, 13>(s, a, M);
     if (n <= 1024 * 16) return launch_row<T, 1024, 16>(s, a, M);
     *done = false;
     hipLaunchKernelGGL((row_stream_kernel<T, 1024>), dim3((unsigned)M), dim3(1024), 0, s, a);
@@ -378,6 +480,8 @@ bool base_ok(const cgn_token_rows* r) {
            (r->dyn_inv_tau || r->inv_tau > 0.f) && (r->M == 0 || (r->logits && r->target));
 }
 
+bool streams(const cgn_token_rows* r) { return r->M * r->V * (r->bf16 ? 2 : 4) >= STREAM_BYTES; }
+
 RowArgs row_args(const cgn_token_rows* r) {
     RowArgs a = {};
     a.logits = r->logits;
@@ -387,13 +491,13 @@ RowArgs row_args(const cgn_token_rows* r) {
     a.V = r->V;
     a.inv_tau = r->inv_tau;
     a.dyn_inv_tau = r->dyn_inv_tau;
-    return a;
+    return a;  // (logits that a second pass will read stay in the caches)
 }
 
 int row_gradient(hipStream_t s, const cgn_token_rows* r, const float* stats, const float* coef, const float* scale,
                  void* dlogits, int64_t ldd) {
     GradArgs g = {r->logits, r->ld, r->target, r->weight, r->V, r->inv_tau, r->dyn_inv_tau, stats, coef, scale, dlogits,
-                  ldd};
+                  ldd, streams(r), 0};
     return run_grad(s, g, r->M, r->bf16 != 0);
 }
 
@@ -445,6 +549,7 @@ extern "C" int cgn_policy_loss(void* stream, const cgn_token_rows* r, const floa
         a.row_loss = row_loss;
         a.dlogits = dlogits;
         a.ldd = ldd;
+        a.stream_in = a.stream_out = dlogits && streams(r);
         bool done;
         int rc = run_rows(s, a, r->M, r->bf16 != 0, &done);
         if (rc == CGN_OK && dlogits && !done) rc = row_gradient(s, r, stats, coef, nullptr, dlogits, ldd);

@@ -206,7 +206,7 @@ PROTOTYPES = {
                                 c_ptr, c_ptr, c_i64, c_ptr, c_i64]),
     "cgn_preference_loss": (c_i32, [c_ptr, C.POINTER(TokenRows), c_i32, c_ptr, c_f64, c_f64, c_ptr, c_ptr, c_ptr, c_ptr,
                                     c_ptr, c_ptr, c_i64, c_ptr, c_i64]),
-    "cgn_grad_norm_workspace": (c_i32, [c_ptr, c_i32, C.POINTER(c_i64)]),
+    "cgn_grad_norm_workspace": (c_i32, [c_ptr, c_i32, c_i32, C.POINTER(c_i64)]),
     "cgn_grad_norm": (c_i32, [c_ptr, c_ptr, c_i32, c_i32, c_f64, c_f64, c_ptr, c_ptr, c_ptr, c_i64]),
     "cgn_clip_grads": (c_i32, [c_ptr, c_ptr, c_i32, c_i32, c_f64, c_f64, c_ptr, c_ptr, c_i64]),
     "cgn_adam_clipped_f32": (c_i32, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_f32, c_f32, c_f32, c_f32, c_i32, c_ptr,

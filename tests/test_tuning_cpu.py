@@ -228,15 +228,23 @@ def test_entry_points_refuse_bad_arguments():
     for t in ((0, 0, 1, 4, 0, 0, 0), (4096, 0, -1, 4, 0, 0, 0), (4096, 0, 2, 4, 3, 4, 0), (4098, 0, 1, 4, 0, 0, 0),
               (4097, 0, 1, 4, 0, 0, 1)):
         tb, n = table(t)
-        assert lib.cgn_grad_norm_workspace(tb, n, C.byref(nb)) == BAD, t
+        assert lib.cgn_grad_norm_workspace(tb, n, 0, C.byref(nb)) == BAD, t
     tb, n = table((4096, 4096, 1, 10 ** 9, 0, 0, 0), (4096, 4096, 300, 825, 828, 828, 0), (0, 0, 1, 0, 0, 0, 0))
-    assert lib.cgn_grad_norm_workspace(tb, n, C.byref(nb)) == _lib.CGN_OK and 8 * 1000 < nb.value < 8 * 2000
+    assert lib.cgn_grad_norm_workspace(tb, n, 0, C.byref(nb)) == _lib.CGN_OK and 8 * 1000 < nb.value < 8 * 2000
     assert lib.cgn_grad_norm(None, tb, n, 0, 1.0, 1.0, P, P, P, 8) == _lib.CGN_ERR_WORKSPACE
     assert lib.cgn_grad_norm(None, tb, n, 0, 1.0, -1.0, P, P, P, nb.value) == BAD
     assert lib.cgn_clip_grads(None, tb, n, 0, 1.0, float("nan"), P, P, nb.value) == BAD
     assert lib.cgn_clip_grads(None, tb, n, 0, 1.0, 1.0, None, P, nb.value) == BAD
     tb, n = table((4096, 0, 1, 4, 0, 0, 0))
     assert lib.cgn_clip_grads(None, tb, n, 0, 1.0, 1.0, P, P, 1 << 20) == BAD  # no destination
+    for second, ok in ((4096 + 16, True), (4096 + 12, False), (4096, False)):  # two tensors of 4, apart or not
+        tb, n = table((4096, 4096, 1, 4, 0, 0, 0), (second, second, 1, 4, 0, 0, 0))
+        assert lib.cgn_grad_norm_workspace(tb, n, 1, C.byref(nb)) == (_lib.CGN_OK if ok else BAD)
+        assert lib.cgn_grad_norm_workspace(tb, n, 0, C.byref(nb)) == _lib.CGN_OK
+    tb, n = table((4096, 4112, 1, 4, 0, 0, 0))
+    assert lib.cgn_grad_norm_workspace(tb, n, 1, C.byref(nb)) == _lib.CGN_OK
+    tb, n = table((4096, 4108, 1, 4, 0, 0, 0))
+    assert lib.cgn_grad_norm_workspace(tb, n, 1, C.byref(nb)) == BAD
     assert lib.cgn_adam_clipped_f32(None, P, P, P, P, 4, 1e-3, 0.9, 0.999, 1e-8, 1, None, 1.0, None) == BAD
 
 

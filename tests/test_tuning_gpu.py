@@ -238,9 +238,9 @@ def check_dlogits(got, want, tol, what):
 
 
 # sizes on both sides of every register variant: pieces of 4 (fp32) / 8 (bf16) elements, 256..1024 threads
-ROW_SIZES = [(1, 1), (5, 2), (3, 7), (4, 8), (7, 9), (2, 1000), (3, 1023), (2, 1024), (2, 1025), (3, 2049), (2, 4097),
-             (2, 8193), (3, 10000), (2, 16385), (2, 20001), (2, 24577), (2, 32769), (1, 49153), (2, 50000), (1, 65537),
-             (1, 98305), (1, 131075)]
+ROW_SIZES = [(1, 1), (5, 2), (3, 7), (4, 8), (7, 9), (9, 63), (9, 71), (2, 1000), (3, 1023), (2, 1024), (2, 1025),
+             (3, 2049), (2, 4097), (2, 8193), (3, 10000), (2, 16385), (2, 20001), (2, 24577), (2, 32769), (1, 40961),
+             (1, 49153), (2, 50000), (1, 57345), (1, 65537), (1, 81921), (1, 98305), (1, 106497), (1, 131075)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -354,8 +354,7 @@ def test_masked_rows_strides_and_bad_values(dev, V, extra, shift, dtype):
     M, inf = 8, float("inf")
     x0, t, A, w, old, ref = make_policy(M, V, dtype, V, dev)
     w[:] = torch.tensor([0.3, 0, 0.2, 0, 0, 0.1, 0, 0], device=dev)
-    d0 = torch.empty_like(x0)
-    loss0, logp0 = ops.policy_loss(x0, t, A, w, old_logp=old, ref_logp=ref, kl_coef=0.1, dlogits=d0)
+    want = policy_ref(x0, t, A, w, old, ref, 0.2, 0.2, 0.1, 1.0)
     dead = w == 0
     bad = torch.tensor([0, float("nan"), 0, inf, -inf, 0, torch.finfo(dtype).min, inf], device=dev).to(dtype)
     x = strided(torch.where(dead[:, None], bad[:, None], x0), extra, shift)
@@ -364,7 +363,9 @@ def test_masked_rows_strides_and_bad_values(dev, V, extra, shift, dtype):
     A2, old2, ref2 = (torch.where(dead, nan, v) for v in (A, old, ref))
     d = strided(torch.full_like(x0, 7.0), extra, shift)
     loss, logp = ops.policy_loss(x, t2, A2, w, old_logp=old2, ref_logp=ref2, kl_coef=0.1, dlogits=d)
-    assert torch.equal(loss, loss0) and torch.equal(logp, logp0) and torch.equal(d, d0)
+    close(logp, want["logp"], torch.where(dead, 0.0, want["band"]), "logp")
+    assert abs(float(loss) - float(want["loss"])) <= want["loss_tol"] + 2 * U * abs(float(want["loss"])), "loss"
+    check_dlogits(d, want["d"], want["d_tol"], "dlogits")
     assert not d[dead].any() and not logp[dead].any()
     flat = d.as_strided((M * (V + extra) + 8,), (1,), d.storage_offset())
     pad = torch.cat([flat[r * (V + extra) + V:(r + 1) * (V + extra)] for r in range(M)] + [flat[M * (V + extra):]])
@@ -517,18 +518,18 @@ def test_long_offsets(dev):
     target[-3:] = t
     w, adv = torch.zeros(M, device=dev), torch.zeros(M, device=dev)
     w[-3:], adv[-3:] = 1.0, A
+    want = policy_ref(tail, t, A, torch.ones(3, device=dev), None, None, 0.2, 0.2, 0.0, 1.0)
     d = torch.full_like(x, 5.0)
     loss, logp = ops.policy_loss(x, target, adv, w, dlogits=d)
-    d0 = torch.empty_like(tail)
-    loss0, logp0 = ops.policy_loss(tail, t, A, torch.ones(3, device=dev), dlogits=d0)
-    assert torch.equal(loss, loss0) and torch.equal(logp[-3:], logp0) and torch.equal(d[-3:], d0)
+    close(logp[-3:], want["logp"], want["band"], "logp")
+    check_dlogits(d[-3:], want["d"], want["d_tol"], "dlogits")
     assert not d[:-3].any()
     _, stats = ops.token_logp(x, target, w)
     coef = torch.zeros(M, device=dev)
-    coef[-3:] = 1
+    coef[-3:] = -A
     d.fill_(5.0)
     ops.token_logp_bwd(x, target, stats, coef, weight=w, dlogits=d)
-    assert torch.equal(d[-3:], ops.token_logp_bwd(tail, t, stats[-3:].contiguous(), coef[-3:].contiguous()))
+    check_dlogits(d[-3:], want["d"], want["d_tol"], "dlogits, second pass")
     assert not d[:-3].any()
 
 
