@@ -38,6 +38,15 @@ struct RowArgs {
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+template <typename T>
+__device__ __forceinline__ float piece_max(const Piece<T>& q, float m) {
+#pragma unroll
+    for (int e = 0; e < Piece<T>::E; e += 2) m = fmaxf(fmaxf(q.get(e), q.get(e + 1)), m);
+    return m;
+}
+// An infinite total (an infinite logit): the row's results are NaN, as log_softmax has them.
+__device__ __forceinline__ float total(float z) { return z < INFINITY ? z : NAN; }
+
 // Everything of a row that is one number. One thread loads it before the row itself and finishes it once the row's
 // maximum and total are known, so that its dependent loads (target, then the target's logit) pass beside the row's.
 struct RowScalars {
@@ -168,9 +177,7 @@ __global__ __launch_bounds__(NT) void row_kernel(const RowArgs a) {
     const float xe = has_edge ? Piece<T>::one(x + ec) : -INFINITY;
     float m = xe;
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int e = 0; e < E; ++e) m = fmaxf(m, q[j].get(e));
+    for (int j = 0; j < NV; ++j) m = piece_max(q[j], m);
     m = wave_max(m);
     if ((threadIdx.x & 63) == 0) red_m[threadIdx.x >> 6] = m;
     __syncthreads();
@@ -196,6 +203,7 @@ __global__ __launch_bounds__(NT) void row_kernel(const RowArgs a) {
     z = 0.f;
 #pragma unroll
     for (int i = 0; i < NW; ++i) z += red_z[i];
+    z = total(z);
     if (threadIdx.x == 0) coef_s = rs.finish(a, row, w, inv_tau, m, z);
     if (!d) return;
     __syncthreads();
@@ -249,9 +257,7 @@ __global__ __launch_bounds__(NT) void row_stream_kernel(const RowArgs a) {
         }
         float mx = m;
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int e = 0; e < E; ++e) mx = fmaxf(mx, q[u].get(e));
+        for (int u = 0; u < U; ++u) mx = piece_max(q[u], mx);
         const float base = mx == -INFINITY ? 0.f : mx;  // (nothing but -inf so far: every term is zero)
         z *= fast_exp2((m - base) * c2);
         m = mx;
@@ -266,7 +272,7 @@ __global__ __launch_bounds__(NT) void row_stream_kernel(const RowArgs a) {
     const float xe = (int)threadIdx.x < cut.edge ? Piece<T>::one(x + cut.edge_col(threadIdx.x)) : -INFINITY;
     const float mb = block_max<NT>(fmaxf(m, xe), red);
     const float mine = m == -INFINITY && z == 0.f ? 0.f : z * fast_exp2((m - mb) * c2);
-    z = block_sum<NT>(mine + fast_exp2((xe - mb) * c2), red);
+    z = total(block_sum<NT>(mine + fast_exp2((xe - mb) * c2), red));
     if (threadIdx.x == 0) {
         RowScalars rs;
         rs.load<T>(a, row);

@@ -400,11 +400,42 @@ def test_banned_tokens(dev, V, dtype):
     assert not d[ban].any() and torch.isfinite(d.float()).all()
     want["d"][ban], want["d_tol"][ban] = 0, 0
     check_dlogits(d, want["d"], want["d_tol"], "dlogits")
+    y = x.clone()
+    y[2, int(t[2]) - 1] = float("inf")  # an infinite logit: NaN, in its row alone
+    _, logp = ops.policy_loss(y, t, A, w, dlogits=d)
+    assert logp[2].isnan() and d[2].isnan().all() and torch.isfinite(logp[[0, 1, 3, 4, 5]]).all()
     x[1] = -float("inf")  # no token is possible: as log_softmax says, NaN
     _, logp = ops.policy_loss(x, t, A, w, dlogits=d)
     assert logp[1].isnan() and d[1].isnan().all() and torch.isfinite(logp[[0, 2, 3, 4, 5]]).all()
     _, logp = ops.policy_loss(x, t, A, w)
     assert logp[1].isnan()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [37, 5001, 140003])
+@pytest.mark.parametrize("base", [-3.0e38, -1.0e30, -2.0e6, 1.0e5, 2.0e6, 1.0e30, 3.0e38])
+def test_rows_far_from_zero(dev, V, base, dtype):
+    """Rows all of whose logits are at one far value (a mask's lowest value among them), and rows spread around it: the
+    log-probabilities are those of the differences, which are exact here."""
+    x = torch.full((3, V), base, device=dev).to(dtype)
+    step = float(torch.nextafter(x[0, 0], torch.zeros((), device=dev, dtype=dtype))) - float(x[0, 0])
+    g = gen(V)
+    n = torch.randint(0, 3, (V,), device=dev, generator=g)
+    x[1] = (x[1].double() + step * n.double()).to(dtype)  # one, two or three neighbouring values
+    x[2, : V // 2] = torch.finfo(dtype).min
+    t = torch.tensor([0, int(n.argmax()), V - 1], device=dev)
+    lp, ls, band = softmax_ref(x, t, 1.0)
+    # a row's differences are exact, so only the exponentials' own roundings are left: |difference| * 2 u each
+    band = 128 * U + 4 * U * lp.abs()
+    logp, stats = ops.token_logp(x, t)
+    close(logp, lp, band + torch.where(lp.abs() > 80, 2 * U * lp.abs(), 0.0), "logp")
+    coef = torch.ones(3, device=dev)
+    want, tol = dlogits_ref(ls, t, coef.double(), 1.0, band, torch.zeros_like(band))
+    tol = tol + 128 * U * ls.exp()
+    check_dlogits(ops.token_logp_bwd(x, t, stats, coef), want, tol, "dlogits")
+    d = torch.empty_like(x)
+    ops.policy_loss(x, t, -coef, dlogits=d)
+    check_dlogits(d, want, tol, "dlogits of the fused pass")
 
 
 def pair_ref(x, t, w, ref, beta, smooth, it):
