@@ -1447,14 +1447,16 @@ def _rows_any(t, name):
     """(bf16?, rows, columns, row stride) of a float32 / bfloat16 tensor seen as rows of its last axis: 2-D with unit
     column stride, or contiguous with any number of axes."""
     b16 = _chk_f32_or_bf16(t, name)
-    if t.dim() == 2:
-        R, C_ = t.shape
-        ld = t.stride(0) if R > 1 else C_
-        _req((t.stride(1) == 1 or C_ == 1) and ld >= C_, "%s must have unit column stride and rows that do not overlap" % name)
-        return b16, R, C_, ld
-    _req(t.dim() >= 1 and t.is_contiguous(), "%s must be 2-D with unit column stride, or contiguous" % name)
-    C_ = t.shape[-1]
-    return b16, (t.numel() // C_ if C_ else 0), C_, C_
+    if t.is_contiguous():
+        if t.dim() == 0:
+            raise ValueError("%s must have at least one axis" % name)
+        C_ = t.shape[-1]
+        return b16, (t.numel() // C_ if C_ else 0), C_, C_
+    _req(t.dim() == 2, "%s must be 2-D with unit column stride, or contiguous" % name)
+    R, C_ = t.shape
+    ld = t.stride(0) if R > 1 else C_
+    _req((t.stride(1) == 1 or C_ == 1) and ld >= C_, "%s must have unit column stride and rows that do not overlap" % name)
+    return b16, R, C_, ld
 
 
 def _vector(t, n, name, dev):
@@ -1502,7 +1504,7 @@ def layer_norm_bwd(dy, x, weight, mean, rstd, dx=None, dweight=None, dbias=None,
     b16, R, Cn, ldx = _layer_norm_rows(x, "x")
     dev = x.device
     _req(dy.shape == x.shape and dy.dtype == x.dtype and dy.device == dev, "dy must be like x")
-    lddy = _rows_any(dy, "dy")[3]
+    lddy = Cn if dy.is_contiguous() else _rows_any(dy, "dy")[3]
     _vector(mean, R, "mean", dev)
     _vector(rstd, R, "rstd", dev)
     if weight is not None:
@@ -1559,11 +1561,7 @@ def _token_rows(logits, target, weight, inv_tau, dyn):
         _req(dyn.numel() >= 1 and dyn.device == dev, "dyn must hold inv_tau")
     inv_tau = float(inv_tau)
     _req(0.0 < inv_tau < float("inf"), "inv_tau must be positive")
-    r = _lib.TokenRows()
-    r.logits, r.ld, r.M, r.target = logits.data_ptr(), ld, M, target.data_ptr()
-    r.weight = weight.data_ptr() if weight is not None else None
-    r.dyn_inv_tau = dyn.data_ptr() if dyn is not None else None
-    r.V, r.bf16, r.inv_tau = V, b16, inv_tau
+    r = _lib.TokenRows(logits.data_ptr(), ld, M, target.data_ptr(), _addr(weight), _addr(dyn), V, b16, inv_tau)
     return r, M, V, ld, dev
 
 

@@ -92,9 +92,10 @@ class CGNStep:
         self.allreduce = allreduce
         self.world_size = world_size
         self.dp = allreduce is not None and (world_size > 1 or force_dp)
-        # bound on the 2-norm of every optimizer group's gradient (averaged over the ranks), None = no clipping (the
-        # reference's behaviour); the last step's norms before clipping are in `grad_norms`, by group, as device tensors
-        self.max_grad_norm = None
+        # bound on the 2-norm of every optimizer group's gradient (averaged over the ranks), None = no clipping; the last
+        # step's norms before clipping are in `grad_norms`, by group, as device tensors. A captured step keeps the bound
+        # it was captured with.
+        self.max_grad_norm = getattr(model.config, "max_grad_norm", None)
         self.grad_norms = {}
         self._pending = {}     # optimizer group -> handles of its gradient all-reduce in flight
         # The encoder group's gradients become final in two waves: the biLSTM's and the mu|logvar head's right behind the

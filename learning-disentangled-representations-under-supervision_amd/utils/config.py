@@ -9,7 +9,8 @@ class Config:
                  kernels=((1, 25), (2, 50), (3, 75), (4, 100), (5, 125), (6, 150)),
                  encoder_rnn_size=600, encoder_num_layers=1, latent_variable_size=1100,
                  decoder_rnn_size=800, decoder_num_layers=2,
-                 sentiment_kernel_size=(3, 4, 5), sentiment_kernel_num=100, sentiment_dropout=0.3, c_size=1):
+                 sentiment_kernel_size=(3, 4, 5), sentiment_kernel_num=100, sentiment_dropout=0.3, c_size=1,
+                 max_grad_norm=None):
         self.learning_rate = learning_rate
         self.max_word_len = int(max_word_len)
         self.max_seq_len = int(max_seq_len) + 1  # go or eos token (config.py:9)
@@ -42,6 +43,11 @@ class Config:
 
         # width of the structured code c; the reference hard-codes 1 (model/generator.py:17,54)
         self.c_size = int(c_size)
+
+        # bound on the 2-norm of every optimizer group's gradient; None = no clipping, as the reference trains
+        self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)
+        if self.max_grad_norm is not None and not self.max_grad_norm >= 0.0:
+            raise ValueError("max_grad_norm must not be negative")
 
         if self.encoder_num_layers != 1:
             raise NotImplementedError("the HIP encoder path implements the reference's 1-layer biLSTM (config.py:21)")

@@ -840,3 +840,94 @@ def test_captured(dev):
         torch.cuda.synchronize()
         for (_, _, outs), want in zip(sets, wants):
             assert all(torch.equal(p, q) for p, q in zip(outs, want)), rep
+
+
+def test_captured_modules(dev):
+    """Forward and backward of the differentiable forms in a graph, replayed on changing inputs; a capture over parameters
+    that a graph built outside of it still holds is refused before anything of it is recorded."""
+    M, H = 24, 300
+    ln = hnn.LayerNorm(H).to(dev)
+    t = torch.randint(0, H, (M,), device=dev, generator=gen(1))
+    A, w = torch.randn(M, device=dev, generator=gen(2)), torch.rand(M, device=dev, generator=gen(3))
+    x = torch.randn(M, H, device=dev, generator=gen(4))
+
+    def step(v):
+        loss, _ = hnn.policy_loss(ln(v), t, A, w)
+        loss.backward()
+        return loss.detach()
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        alive = ln(x)  # an eager graph over the same parameters
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="alive"):
+            with torch.cuda.graph(graph, stream=side):
+                ln(x)
+        del alive
+        torch.cuda.synchronize()
+        static = x.clone()
+        graph = torch.cuda.CUDAGraph()
+        with ops.capture_without_gc():
+            with torch.cuda.graph(graph, stream=side):
+                out = step(static)
+    torch.cuda.synchronize()
+    grads = [ln.weight.grad, ln.bias.grad]
+    for rep in range(4):
+        new = torch.randn(M, H, device=dev, generator=gen(20 + rep))
+        twin = hnn.LayerNorm(H).to(dev)  # the eager answer, on parameters of its own
+        loss, _ = hnn.policy_loss(twin(new), t, A, w)
+        loss.backward()
+        static.copy_(new)
+        for gr in grads:
+            gr.zero_()  # (the captured accumulation adds where it did not create)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, loss.detach())
+        assert torch.equal(grads[0], twin.weight.grad) and torch.equal(grads[1], twin.bias.grad)
+
+
+def small_engine(dev, **kw):
+    from ldrs_amd.model.cgn import Controlled_Generation_Sentence
+    from ldrs_amd.utils.config import Config
+    from oracle import cgn_oracle as O
+    dims = dict(word_embed_size=12, kernels=((1, 3), (2, 5), (3, 4)), encoder_rnn_size=16, latent_variable_size=6,
+                decoder_rnn_size=20, sentiment_kernel_size=(3, 4, 5), sentiment_kernel_num=6)
+    ocfg = O.OracleConfig(max_word_len=7, max_seq_len=5, word_vocab_size=50, char_vocab_size=20, **dims)
+    torch.manual_seed(2)
+    model = Controlled_Generation_Sentence(Config(7, 5, 50, 20, 1e-3, 7.9, 0.1, 0.1, 1.0, **dims, **kw),
+                                           O.synthetic_word_embed(ocfg)).to(dev)
+    eng = model.step_engine()
+    data = {k: v.to(dev).contiguous() for k, v in O.synthetic_batch(ocfg, 4, 5, seed=1).items()}
+    return model, eng, {g: eng.new_optimizer(g) for g in ("disc", "enc", "gen")}, data
+
+
+def test_training_step_is_clipped(dev):
+    """Config(max_grad_norm=...): the wake-sleep step clips every optimizer group, eager and replayed from a graph."""
+    from ldrs_amd.hip.graph import GraphedWakeSleep
+    plain, wide, tight = small_engine(dev), small_engine(dev, max_grad_norm=1e6), small_engine(dev, max_grad_norm=0.01)
+    for _, eng, opts, data in (plain, wide, tight):
+        eng.wake_sleep(opts, data, 0.5, 0.9)
+    for (n, p), (_, q) in zip(plain[0].named_parameters(), wide[0].named_parameters()):
+        assert torch.equal(p, q), n  # a bound that nothing reaches changes no bit
+    for g in ("disc", "enc", "gen"):
+        grads = [t for t in tight[1].arenas[g].grads.values()]
+        want = norm64(grads)
+        assert want > 0.01 and abs(float(tight[1].grad_norms[g]) - want) <= 2 * U * want
+        # first step: m = (1 - beta1) * clipped gradient
+        m = float(tight[2][g].m.double().norm())
+        assert abs(m - 0.1 * 0.01) <= 1e-6 * 0.1 * 0.01 + 0.1 * 0.01 * 1e-6 / want
+    assert not plain[1].grad_norms
+    eager, graphed = small_engine(dev, max_grad_norm=0.01), small_engine(dev, max_grad_norm=0.01)
+    for _ in range(4):
+        eager[1].wake_sleep(eager[2], eager[3], 0.5, 0.9)
+    rep = GraphedWakeSleep(graphed[1], graphed[2], graphed[3], warmup_kld=0.5, warmup_tau=0.9)
+    for _ in range(3):
+        rep(0.5, 0.9, graphed[3])
+        torch.cuda.synchronize()
+    for (n, p), (_, q) in zip(eager[0].named_parameters(), graphed[0].named_parameters()):
+        err = (p - q).abs().max().item() / max(p.abs().max().item(), 1e-12)
+        assert err <= 2e-6, (n, err)  # (the bias corrections are formed on the device there)
+    with pytest.raises(ValueError):
+        small_engine(dev, max_grad_norm=-1.0)
