@@ -47,8 +47,10 @@ __device__ __forceinline__ float piece_max(const Piece<T>& q, float m) {
 // An infinite total (an infinite logit): the row's results are NaN, as log_softmax has them.
 __device__ __forceinline__ float total(float z) { return z < INFINITY ? z : NAN; }
 
-// Everything of a row that is one number. One thread loads it before the row itself and finishes it once the row's
-// maximum and total are known, so that its dependent loads (target, then the target's logit) pass beside the row's.
+// Everything of a row that is one number, in the hands of one thread: loaded before the row itself, so that the dependent
+// loads (target, then the target's logit) pass beside the row's; then, with the row's maximum and total, first the factor
+// that the workgroup waits for, in fp32, and at the end, behind the gradient's stores, what is written out, in 64 bits: a
+// loss is a sum of terms of both signs, where the roundings of logf and expf would show.
 struct RowScalars {
     float xt, A, old_logp, ref_logp;
 
@@ -62,30 +64,37 @@ struct RowScalars {
         xt = t >= 0 && t < a.V ? Piece<T>::one((const T*)a.logits + row * a.ld + t) : NAN;
     }
 
-    // writes the row's results; returns d loss / d lp
-    __device__ __forceinline__ float finish(const RowArgs& a, long row, float w, float inv_tau, float m, float z) const {
+    // d loss / d lp. expm1: k is small where the two policies agree.
+    __device__ __forceinline__ float slope(const RowArgs& a, float w, float inv_tau, float m, float z) const {
         const double lp = ((double)xt - (double)m) * (double)inv_tau - (double)logf(z);
+        const float ratio = a.old_logp ? expf((float)(lp - (double)old_logp)) : 1.f;
+        const bool cut = (A > 0.f && ratio > 1.f + a.clip_hi) || (A < 0.f && ratio < 1.f - a.clip_lo);
+        float g = cut ? 0.f : -ratio * A;
+        if (a.ref_logp) g -= a.kl_coef * expm1f((float)((double)ref_logp - lp));
+        return g * w;
+    }
+
+    __device__ __forceinline__ void write(const RowArgs& a, long row, float w, float inv_tau, float m, float z,
+                                          float g) const {
+        const double lp = ((double)xt - (double)m) * (double)inv_tau - log((double)z);
         if (a.logp) a.logp[row] = (float)lp;
         if (a.lp64) a.lp64[row] = lp * (double)w;
         if (a.stats) {
             a.stats[2 * row] = m;
             a.stats[2 * row + 1] = z;
         }
-        if (!a.advantage) return 0.f;
-        const float ratio = a.old_logp ? expf((float)(lp - (double)old_logp)) : 1.f;
-        const float lim = fminf(fmaxf(ratio, 1.f - a.clip_lo), 1.f + a.clip_hi);
-        const bool cut = (A > 0.f && ratio > 1.f + a.clip_hi) || (A < 0.f && ratio < 1.f - a.clip_lo);
-        float loss = -(cut ? lim : ratio) * A, g = cut ? 0.f : -ratio * A;
-        if (a.ref_logp) {
-            // exp(k) - k - 1 and its derivative through expm1: k is small where the two policies agree
-            const float k = (float)((double)ref_logp - lp), e = expm1f(k);
-            loss += a.kl_coef * (e - k);
-            g -= a.kl_coef * e;
-        }
-        a.row_loss[row] = (double)loss * (double)w;
-        g *= w;
+        if (!a.advantage) return;
         if (a.coef) a.coef[row] = g;
-        return g;
+        const double ratio = a.old_logp ? exp(lp - (double)old_logp) : 1.0;
+        const double lo = 1.0 - (double)a.clip_lo, hi = 1.0 + (double)a.clip_hi;
+        // the smaller of ratio A and clip(ratio) A
+        const double kept = A > 0.f ? (ratio > hi ? hi : ratio) : (ratio < lo ? lo : ratio);
+        double loss = -kept * (double)A;
+        if (a.ref_logp) {
+            const double k = (double)ref_logp - lp;
+            loss += (double)a.kl_coef * (expm1(k) - k);
+        }
+        a.row_loss[row] = loss * (double)w;
     }
 };
 
@@ -204,8 +213,13 @@ __global__ __launch_bounds__(NT) void row_kernel(const RowArgs a) {
 #pragma unroll
     for (int i = 0; i < NW; ++i) z += red_z[i];
     z = total(z);
-    if (threadIdx.x == 0) coef_s = rs.finish(a, row, w, inv_tau, m, z);
-    if (!d) return;
+    float g = 0.f;
+    if (threadIdx.x == 0 && a.advantage) g = rs.slope(a, w, inv_tau, m, z);
+    if (!d) {
+        if (threadIdx.x == 0) rs.write(a, row, w, inv_tau, m, z, g);
+        return;
+    }
+    if (threadIdx.x == 0) coef_s = g;
     __syncthreads();
     keep_packed<T, NV>(q);
     const float c = coef_s * inv_tau, cz = -c / z;
@@ -227,6 +241,7 @@ __global__ __launch_bounds__(NT) void row_kernel(const RowArgs a) {
         }
     }
     if (has_edge) Piece<T>::put(d + ec, pe * cz + (ec == t ? c : 0.f));
+    if (threadIdx.x == 0) rs.write(a, row, w, inv_tau, m, z, g);
 }
 
 // A row too long for the registers of a workgroup: running maximum and total per thread, joined at the end.
@@ -276,7 +291,7 @@ __global__ __launch_bounds__(NT) void row_stream_kernel(const RowArgs a) {
     if (threadIdx.x == 0) {
         RowScalars rs;
         rs.load<T>(a, row);
-        rs.finish(a, row, w, inv_tau, mb, z);
+        rs.write(a, row, w, inv_tau, mb, z, a.advantage ? rs.slope(a, w, inv_tau, mb, z) : 0.f);
     }
 }
 
