@@ -617,7 +617,8 @@ int cgn_layer_norm_fwd(void* stream, const void* x, int64_t ldx, int64_t R, int3
                        const float* bias, float eps, void* y, int64_t ldy, float* mean, float* rstd);
 /* Its backward pass, from the statistics of the forward pass: dx (nullable; may be dy's or x's own buffer) and
  * dweight / dbias = beta * itself + the sums over the rows (nullable; R == 0 gives sums of zero).
- * workspace (with dweight or dbias): min(R, 1024) * 2 * C * 4 bytes. */
+ * workspace (with dweight or dbias): what cgn_layer_norm_bwd_workspace says for the shape (host call; may be nothing). */
+int cgn_layer_norm_bwd_workspace(int64_t R, int32_t C, int32_t bf16, int64_t* bytes);
 int cgn_layer_norm_bwd(void* stream, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t R, int32_t C,
                        int32_t bf16, const float* weight, const float* mean, const float* rstd, void* dx, int64_t lddx,
                        float* dweight, float* dbias, float beta, float* workspace, int64_t workspace_bytes);

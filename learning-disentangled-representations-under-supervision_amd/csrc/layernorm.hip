@@ -152,7 +152,8 @@ template <typename T, int NT, int G, int NV>
 __global__ __launch_bounds__(NT) void layer_norm_bwd_kernel(const T* dy, long lddy, const T* x, long ldx, long R, int C,
                                                             const float* __restrict__ w, const float* __restrict__ mean,
                                                             const float* __restrict__ rstd, T* dx, long lddx,
-                                                            float* __restrict__ part, bool stream) {
+                                                            float* __restrict__ part, float* dw, float* db, float beta,
+                                                            bool stream) {
     constexpr int E = Piece<T>::E;
     constexpr int GROUPS = NT / G;
     __shared__ float red[NT / 64 * 3];
@@ -233,9 +234,15 @@ __global__ __launch_bounds__(NT) void layer_norm_bwd_kernel(const T* dy, long ld
             if (dx) Piece<T>::put(dx + r * lddx + nfull * E + lane, fmaf(gt, rs, fmaf(xht - off, cx, c0)));
         }
     }
-    if (!part) return;
+    if (!part && !dw && !db) return;
     // the workgroup's groups summed in a fixed order, one piece of every lane at a time through LDS
-    float* out = part + (long)blockIdx.x * 2 * C;
+    const auto put = [&](int k, int c, float v) {
+        if (part) {
+            part[((long)blockIdx.x * 2 + k) * C + c] = v;
+        } else if (float* o = k ? db : dw) {  // the only workgroup: nothing is left to be reduced
+            o[c] = beta != 0.f ? v + beta * o[c] : v;
+        }
+    };
     __shared__ float rows[GROUPS][GROUPS > 1 ? G * E : 1];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -250,7 +257,7 @@ __global__ __launch_bounds__(NT) void layer_norm_bwd_kernel(const T* dy, long ld
                     if (e >= width) break;
                     const int c = col0 + lane * width + e;
                     const float v = j < NV ? (k ? ab[j < NV ? j : 0][e] : aw[j < NV ? j : 0][e]) : (k ? abt : awt);
-                    if (c < cend) out[k * C + c] = v;
+                    if (c < cend) put(k, c, v);
                 }
             } else {
                 __syncthreads();
@@ -265,7 +272,7 @@ __global__ __launch_bounds__(NT) void layer_norm_bwd_kernel(const T* dy, long ld
                     float t = 0.f;
 #pragma unroll
                     for (int q = 0; q < GROUPS; ++q) t += rows[q][c];
-                    if (col0 + c < cend) out[k * C + col0 + c] = t;
+                    if (col0 + c < cend) put(k, col0 + c, t);
                 }
             }
         }
@@ -299,6 +306,7 @@ __global__ __launch_bounds__(LNF_NT) void layer_norm_params_kernel(const float* 
 }
 
 constexpr int LN_MAX_C = 8192;    // widest row that the groups below hold in registers
+constexpr int LN_ALONE = 4;       // a backward pass of that many workgroups' rows is left to one
 constexpr int LN_FWD_NB = 8192;   // workgroups of a forward pass at most: each with many rows behind one read of w and b
 
 template <typename T, int NT, int G, int NV>
@@ -313,23 +321,33 @@ int launch_fwd(hipStream_t s, const void* x, int64_t ldx, int64_t R, int C, cons
     return CGN_OK;
 }
 
-// WAVES: waves per CU that the variant's registers leave room for; as many workgroups walk the rows, and leave a row of
-// `part` each (more would only lengthen the reduction behind them).
+// Workgroups of a backward pass. WAVES: waves per CU that the variant's registers leave room for; as many workgroups walk
+// the rows, and leave a row of `part` each (more would only lengthen the reduction behind them). A few rows take one
+// workgroup, which needs no reduction: at 16 x 800 that is one launch of 5 us instead of two of 3 and 4 us.
+template <int NT, int G, int WAVES>
+int64_t bwd_blocks(int64_t R) {
+    const int64_t per = NT / G, nb = (R + per - 1) / per, most = 256 * WAVES * 64 / NT;
+    return nb <= LN_ALONE ? (nb > 0) : nb > most ? most : nb;
+}
+
 template <typename T, int NT, int G, int NV, int WAVES>
 int launch_bwd(hipStream_t s, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t R, int C, const float* w,
                const float* mean, const float* rstd, void* dx, int64_t lddx, float* dw, float* db, float beta,
-               float* part, int64_t part_bytes) {
-    int64_t nb = (R + NT / G - 1) / (NT / G);
-    if (nb > 256 * WAVES * 64 / NT) nb = 256 * WAVES * 64 / NT;
-    const bool params = dw || db;
-    if (params && nb * 2 * C * 4 > part_bytes) return CGN_ERR_WORKSPACE;
+               float* part, int64_t part_bytes, int64_t* need) {
+    const int64_t nb = bwd_blocks<NT, G, WAVES>(R);
+    const bool params = dw || db, alone = nb == 1;
+    if (need) {
+        *need = alone ? 0 : nb * 2 * C * 4;
+        return CGN_OK;
+    }
+    if (params && !alone && nb * 2 * C * 4 > part_bytes) return CGN_ERR_WORKSPACE;
     if (nb > 0) {
         hipLaunchKernelGGL((layer_norm_bwd_kernel<T, NT, G, NV>), dim3((unsigned)nb), dim3(NT), 0, s, (const T*)dy,
                            (long)lddy, (const T*)x, (long)ldx, (long)R, C, w, mean, rstd, (T*)dx, (long)lddx,
-                           params ? part : nullptr, R * C * (int64_t)sizeof(T) >= STREAM_BYTES);
+                           params && !alone ? part : nullptr, dw, db, beta, R * C * (int64_t)sizeof(T) >= STREAM_BYTES);
         CGN_LAUNCH_CHECK();
     }
-    if (params) {
+    if (params && !alone) {
         hipLaunchKernelGGL(layer_norm_params_kernel, dim3(cgn_cdiv(2L * C, 64)), dim3(LNF_NT), 0, s, part, (int)nb, C, beta,
                            dw, db);
         CGN_LAUNCH_CHECK();
@@ -368,11 +386,11 @@ int norm_fwd(hipStream_t s, const void* x, int64_t ldx, int64_t R, int C, const 
 template <typename T>
 int norm_bwd(hipStream_t s, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t R, int C, const float* w,
              const float* mean, const float* rstd, void* dx, int64_t lddx, float* dw, float* db, float beta, float* part,
-             int64_t part_bytes) {
+             int64_t part_bytes, int64_t* need) {
     const int n = cgn_cdiv(C, Piece<T>::E);
 #define LN_BWD(NT, G, NV, WAVES)                                                                                       \
     return launch_bwd<T, NT, G, NV, WAVES>(s, dy, lddy, x, ldx, R, C, w, mean, rstd, dx, lddx, dw, db, beta, part,     \
-                                           part_bytes)
+                                           part_bytes, need)
     if (n <= 8) LN_BWD(512, 8, 1, 16);
     if (n <= 16) LN_BWD(512, 16, 1, 16);
     if (n <= 32) LN_BWD(512, 32, 1, 16);
@@ -405,16 +423,24 @@ extern "C" int cgn_layer_norm_fwd(void* stream, const void* x, int64_t ldx, int6
                 : norm_fwd<float>(s, x, ldx, R, C, weight, bias, eps, y, ldy, mean, rstd);
 }
 
+extern "C" int cgn_layer_norm_bwd_workspace(int64_t R, int32_t C, int32_t bf16, int64_t* bytes) {
+    CGN_CHECK_ARG(R >= 0 && C > 0 && C <= LN_MAX_C && bytes);
+    return bf16 ? norm_bwd<Bf16>(nullptr, nullptr, C, nullptr, C, R, C, nullptr, nullptr, nullptr, nullptr, C, nullptr,
+                                 nullptr, 0.f, nullptr, 0, bytes)
+                : norm_bwd<float>(nullptr, nullptr, C, nullptr, C, R, C, nullptr, nullptr, nullptr, nullptr, C, nullptr,
+                                  nullptr, 0.f, nullptr, 0, bytes);
+}
+
 extern "C" int cgn_layer_norm_bwd(void* stream, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t R,
                                   int32_t C, int32_t bf16, const float* weight, const float* mean, const float* rstd,
                                   void* dx, int64_t lddx, float* dweight, float* dbias, float beta, float* workspace,
                                   int64_t workspace_bytes) {
     CGN_CHECK_ARG(R >= 0 && C > 0 && C <= LN_MAX_C && lddy >= C && ldx >= C && (!dx || lddx >= C));
     CGN_CHECK_ARG(R == 0 || (dy && x && mean && rstd));
-    CGN_CHECK_ARG((!dweight && !dbias) || R == 0 || workspace);
+    CGN_CHECK_ARG((!dweight && !dbias) || workspace || workspace_bytes == 0);
     hipStream_t s = (hipStream_t)stream;
     return bf16 ? norm_bwd<Bf16>(s, dy, lddy, x, ldx, R, C, weight, mean, rstd, dx, lddx, dweight, dbias, beta, workspace,
-                                 workspace_bytes)
+                                 workspace_bytes, nullptr)
                 : norm_bwd<float>(s, dy, lddy, x, ldx, R, C, weight, mean, rstd, dx, lddx, dweight, dbias, beta,
-                                  workspace, workspace_bytes);
+                                  workspace, workspace_bytes, nullptr);
 }

@@ -198,6 +198,7 @@ PROTOTYPES = {
     "cgn_gemm_bb_wants": (c_i32, [c_i32, c_i32, c_i32]),
     "cgn_layer_norm_fwd": (c_i32, [c_ptr, c_ptr, c_i64, c_i64, c_i32, c_i32, c_ptr, c_ptr, c_f32, c_ptr, c_i64, c_ptr,
                                    c_ptr]),
+    "cgn_layer_norm_bwd_workspace": (c_i32, [c_i64, c_i32, c_i32, C.POINTER(c_i64)]),
     "cgn_layer_norm_bwd": (c_i32, [c_ptr, c_ptr, c_i64, c_ptr, c_i64, c_i64, c_i32, c_i32, c_ptr, c_ptr, c_ptr, c_ptr,
                                    c_i64, c_ptr, c_ptr, c_f32, c_ptr, c_i64]),
     "cgn_token_logp": (c_i32, [c_ptr, C.POINTER(TokenRows), c_ptr, c_ptr]),

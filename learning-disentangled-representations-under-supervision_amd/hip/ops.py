@@ -609,12 +609,13 @@ def _call(name, dev, *args):
     the current one, and the stream handle is read without making a Stream object: 4 us less host time per call."""
     fn = getattr(_lib.load(), name)
     idx = dev.index
-    if idx is None or idx != torch.cuda.current_device():
+    if idx is None or idx != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
             rc = fn(_stream(), *args)
     else:
         rc = fn(torch._C._cuda_getCurrentRawStream(idx), *args)
-    _lib.check(rc, name)
+    if rc:
+        _lib.check(rc, name)
 
 
 def _req(cond, msg):
@@ -1532,7 +1533,10 @@ def layer_norm_bwd(dy, x, weight, mean, rstd, dx=None, dweight=None, dbias=None,
                 _vector(dbias, Cn, "dbias", dev)
             else:
                 dbias = alloc((Cn,), dev)
-        ws = alloc((min(R, 1024) * 2 * Cn,), dev)
+        nb = C.c_int64()
+        _lib.check(_lib.load().cgn_layer_norm_bwd_workspace(R, Cn, b16, C.byref(nb)), "cgn_layer_norm_bwd_workspace")
+        if nb.value:
+            ws = alloc((nb.value // 4,), dev)
     else:
         _req(dweight is None and dbias is None, "params=False takes no destinations for the parameters")
     _call("cgn_layer_norm_bwd", dev, dy.data_ptr(), lddy, x.data_ptr(), ldx, R, Cn, b16, _addr(weight), mean.data_ptr(),
@@ -1649,7 +1653,7 @@ def preference_loss(logits, target, weight, ref_logp, *, beta, label_smoothing=0
     beta, label_smoothing = float(beta), float(label_smoothing)
     _req(0.0 < beta < float("inf") and 0.0 <= label_smoothing < 0.5, "beta > 0 and 0 <= label_smoothing < 0.5")
     ldd = 0 if dlogits is None else _dlogits_dest(logits, ld, dlogits)
-    loss, margin, seq_logp = alloc((1,), dev), alloc((S // 2,), dev), alloc((S,), dev)
+    loss, margin, seq_logp = alloc((1 + S // 2 + S,), dev).split((1, S // 2, S))
     stats, coef = (alloc((M, 2), dev), alloc((M,), dev)) if save else (None, None)
     ws = alloc((3 * M + 2,), dev, torch.float64)
     _call("cgn_preference_loss", dev, C.byref(r), T, ref_logp.data_ptr(), beta, label_smoothing, loss.data_ptr(),

@@ -186,10 +186,16 @@ def test_entry_points_refuse_bad_arguments():
               dict(mean=None), dict(eps=-1.0)):
         assert ln(**k) == BAD, k
     assert ln(R=0) == _lib.CGN_OK
-    lb = lambda **k: lib.cgn_layer_norm_bwd(None, P, 8, P, 8, 2, 8, 0, None, k.get("mean", P), P, P, k.get("lddx", 8),  # noqa: E731
+    lb = lambda **k: lib.cgn_layer_norm_bwd(None, P, 8, P, 8, 2000, 8, 0, None, k.get("mean", P), P, P, k.get("lddx", 8),  # noqa: E731
                                             P, P, 0.0, k.get("ws", P), k.get("bytes", 1 << 20))
     assert lb(mean=None) == BAD and lb(lddx=7) == BAD and lb(ws=None) == BAD
-    assert lb(bytes=60) == _lib.CGN_ERR_WORKSPACE
+    nb = C.c_int64()
+    assert lib.cgn_layer_norm_bwd_workspace(2000, 8, 0, C.byref(nb)) == _lib.CGN_OK and nb.value > 0
+    assert lb(bytes=nb.value - 1) == _lib.CGN_ERR_WORKSPACE and lb(ws=None, bytes=0) == _lib.CGN_ERR_WORKSPACE
+    assert lib.cgn_layer_norm_bwd_workspace(3, 8, 0, C.byref(nb)) == _lib.CGN_OK and nb.value == 0
+    assert lib.cgn_layer_norm_bwd_workspace(0, 8, 0, C.byref(nb)) == _lib.CGN_OK and nb.value == 0
+    for k in ((-1, 8), (2, 0), (2, 8193)):
+        assert lib.cgn_layer_norm_bwd_workspace(*k, 0, C.byref(nb)) == BAD
 
     def rows(**k):
         r = _lib.TokenRows()

@@ -72,7 +72,8 @@ def norm_ref(x, w, b, eps, dy=None):
 
 NORM_SIZES = [(1, 1), (3, 1), (1, 2), (5, 7), (2, 8), (33, 9), (64, 33), (7, 63), (9, 64), (4, 65), (130, 127), (3, 256),
               (5, 257), (3, 300), (65, 512), (6, 513), (4, 600), (10, 800), (37, 825), (300, 1024), (5, 1025), (2, 2047),
-              (3, 2049), (2, 4096), (3, 4097), (2, 8191), (2, 8192), (2100, 40)]
+              (3, 2049), (2, 4096), (3, 4097), (2, 8191), (2, 8192), (2100, 40), (7, 1500), (9, 3000),
+              (11, 8000), (40, 500), (700, 20)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -464,7 +465,7 @@ def pair_ref(x, t, w, ref, beta, smooth, it):
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("P,T,V", [(1, 1, 5), (1, 3, 1000), (3, 1, 33), (2, 65, 77), (5, 21, 300), (2, 7, 20001),
-                                   (1, 2, 131075), (70, 3, 40)])
+                                   (1, 2, 131075), (70, 3, 40), (70, 65, 9)])
 def test_preference_loss(dev, P, T, V, dtype):
     x, t, g = make_rows(2 * P * T, V, dtype, P * 1009 + T * 101 + V, dev)
     n = torch.randint(0, T + 1, (2 * P, 1), device=dev, generator=g)
