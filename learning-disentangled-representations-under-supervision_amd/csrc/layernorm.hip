@@ -417,7 +417,7 @@ extern "C" int cgn_layer_norm_fwd(void* stream, const void* x, int64_t ldx, int6
                                   float* rstd) {
     CGN_CHECK_ARG(R >= 0 && C > 0 && C <= LN_MAX_C && ldx >= C && ldy >= C && eps >= 0.f);
     if (R == 0) return CGN_OK;
-    CGN_CHECK_ARG(x && y && mean && rstd);
+    CGN_CHECK_ARG(x && y && mean && rstd && ((uintptr_t)x | (uintptr_t)y) % (bf16 ? 2 : 4) == 0);
     hipStream_t s = (hipStream_t)stream;
     return bf16 ? norm_fwd<Bf16>(s, x, ldx, R, C, weight, bias, eps, y, ldy, mean, rstd)
                 : norm_fwd<float>(s, x, ldx, R, C, weight, bias, eps, y, ldy, mean, rstd);
@@ -437,6 +437,7 @@ extern "C" int cgn_layer_norm_bwd(void* stream, const void* dy, int64_t lddy, co
                                   int64_t workspace_bytes) {
     CGN_CHECK_ARG(R >= 0 && C > 0 && C <= LN_MAX_C && lddy >= C && ldx >= C && (!dx || lddx >= C));
     CGN_CHECK_ARG(R == 0 || (dy && x && mean && rstd));
+    CGN_CHECK_ARG(((uintptr_t)dy | (uintptr_t)x | (uintptr_t)dx) % (bf16 ? 2 : 4) == 0);
     CGN_CHECK_ARG((!dweight && !dbias) || workspace || workspace_bytes == 0);
     hipStream_t s = (hipStream_t)stream;
     return bf16 ? norm_bwd<Bf16>(s, dy, lddy, x, ldx, R, C, weight, mean, rstd, dx, lddx, dweight, dbias, beta, workspace,

@@ -343,9 +343,9 @@ __global__ __launch_bounds__(NT) void row_grad_kernel(const GradArgs a) {
     const float xe = has_edge ? Piece<T>::one(x + ec) : 0.f;
     const float inv_tau = a.dyn_inv_tau ? a.dyn_inv_tau[0] : a.inv_tau;
     const float c2 = inv_tau * LOG2E, m = a.stats[2 * row], z = a.stats[2 * row + 1];
-    const float c = a.coef[row] * (a.scale ? a.scale[0] : 1.f) * inv_tau, cz = -c / z;
     const int64_t t64 = a.target[row];
     const int t = t64 >= 0 && t64 < a.V ? (int)t64 : -1;
+    const float c = t < 0 ? NAN : a.coef[row] * (a.scale ? a.scale[0] : 1.f) * inv_tau, cz = -c / z;
     const int tp = t < cut.head ? -1 : (t - cut.head) / E, te = t - cut.head - tp * E;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -438,10 +438,33 @@ __global__ __launch_bounds__(PAIR_NT) void pair_kernel(const double* __restrict_
     }
 }
 
+// The rows from r0 on.
+template <typename T>
+RowArgs rows_from(RowArgs a, int64_t r0) {
+    a.logits = (const T*)a.logits + r0 * a.ld;
+    a.target += r0;
+    if (a.weight) a.weight += r0;
+    if (a.logp) a.logp += r0;
+    if (a.lp64) a.lp64 += r0;
+    if (a.stats) a.stats += 2 * r0;
+    if (a.advantage) a.advantage += r0;
+    if (a.old_logp) a.old_logp += r0;
+    if (a.ref_logp) a.ref_logp += r0;
+    if (a.row_loss) a.row_loss += r0;
+    if (a.coef) a.coef += r0;
+    if (a.dlogits) a.dlogits = (T*)a.dlogits + r0 * a.ldd;
+    return a;
+}
+
+constexpr int64_t GRID_THREADS = 1LL << 31;  // threads of one launch (the hardware counts them in 32 bits)
+
 template <typename T, int NT, int NV>
 int launch_row(hipStream_t s, const RowArgs& a, int64_t M) {
-    hipLaunchKernelGGL((row_kernel<T, NT, NV>), dim3((unsigned)M), dim3(NT), 0, s, a);
-    CGN_LAUNCH_CHECK();
+    for (int64_t r = 0; r < M; r += GRID_THREADS / NT) {
+        const int64_t n = M - r < GRID_THREADS / NT ? M - r : GRID_THREADS / NT;
+        hipLaunchKernelGGL((row_kernel<T, NT, NV>), dim3((unsigned)n), dim3(NT), 0, s, rows_from<T>(a, r));
+        CGN_LAUNCH_CHECK();
+    }
     return CGN_OK;
 }
 
@@ -450,7 +473,7 @@ int launch_grad(hipStream_t s, GradArgs g, int64_t M) {
     constexpr int NT = 256, U = 2;
     g.chunks = cgn_cdiv(g.V, (long)Piece<T>::E * NT * U);
     // whole rows per launch, as many as a grid holds
-    const int64_t most = 0x7fffffff / g.chunks;
+    const int64_t most = GRID_THREADS / NT / g.chunks;
     for (int64_t r = M; r > 0; r -= most) {
         const int64_t n = r < most ? r : most, r0 = r - n;
         GradArgs b = g;
@@ -487,8 +510,11 @@ int launch_rows(hipStream_t s, RowArgs a, int64_t M, bool* done) {
     if (n <= 1024 * 13) return launch_row<T, 1024, 13>(s, a, M);
     if (n <= 1024 * 16) return launch_row<T, 1024, 16>(s, a, M);
     *done = false;
-    hipLaunchKernelGGL((row_stream_kernel<T, 1024>), dim3((unsigned)M), dim3(1024), 0, s, a);
-    CGN_LAUNCH_CHECK();
+    for (int64_t r = 0; r < M; r += GRID_THREADS / 1024) {
+        const int64_t m = M - r < GRID_THREADS / 1024 ? M - r : GRID_THREADS / 1024;
+        hipLaunchKernelGGL((row_stream_kernel<T, 1024>), dim3((unsigned)m), dim3(1024), 0, s, rows_from<T>(a, r));
+        CGN_LAUNCH_CHECK();
+    }
     return CGN_OK;
 }
 
@@ -508,7 +534,13 @@ int run_sum(hipStream_t s, const double* v, int64_t n, double scale, float* out)
 
 bool base_ok(const cgn_token_rows* r) {
     return r && r->M >= 0 && r->M <= 0x7fffffff && r->V > 0 && r->ld >= r->V &&
-           (r->dyn_inv_tau || r->inv_tau > 0.f) && (r->M == 0 || (r->logits && r->target));
+           (r->dyn_inv_tau || r->inv_tau > 0.f) && (r->M == 0 || (r->logits && r->target)) &&
+           (uintptr_t)r->logits % (r->bf16 ? 2 : 4) == 0;
+}
+
+// (element-aligned: what the row kernels' accesses take)
+bool dest_ok(const cgn_token_rows* r, const void* d, int64_t ldd) {
+    return ldd >= r->V && (uintptr_t)d % (r->bf16 ? 2 : 4) == 0;
 }
 
 bool streams(const cgn_token_rows* r) { return r->M * r->V * (r->bf16 ? 2 : 4) >= STREAM_BYTES; }
@@ -547,7 +579,7 @@ extern "C" int cgn_token_logp(void* stream, const cgn_token_rows* r, float* logp
 
 extern "C" int cgn_token_logp_bwd(void* stream, const cgn_token_rows* r, const float* stats, const float* coef,
                                   const float* scale, void* dlogits, int64_t ldd) {
-    CGN_CHECK_ARG(base_ok(r) && ldd >= r->V);
+    CGN_CHECK_ARG(base_ok(r) && dest_ok(r, dlogits, ldd));
     if (r->M == 0) return CGN_OK;
     CGN_CHECK_ARG(stats && coef && dlogits);
     return row_gradient((hipStream_t)stream, r, stats, coef, scale, dlogits, ldd);
@@ -557,7 +589,7 @@ extern "C" int cgn_policy_loss(void* stream, const cgn_token_rows* r, const floa
                                const float* ref_logp, float clip_lo, float clip_hi, float kl_coef, float* loss,
                                float* logp, float* stats, float* coef, void* dlogits, int64_t ldd, void* workspace,
                                int64_t workspace_bytes) {
-    CGN_CHECK_ARG(base_ok(r) && loss && clip_lo >= 0.f && clip_hi >= 0.f && (!dlogits || ldd >= r->V));
+    CGN_CHECK_ARG(base_ok(r) && loss && clip_lo >= 0.f && clip_hi >= 0.f && (!dlogits || dest_ok(r, dlogits, ldd)));
     CGN_CHECK_ARG(r->M == 0 || (advantage && logp && workspace && (uintptr_t)workspace % 8 == 0));
     if (r->M * 24 + 16 > workspace_bytes) return CGN_ERR_WORKSPACE;
     hipStream_t s = (hipStream_t)stream;
@@ -594,7 +626,7 @@ extern "C" int cgn_preference_loss(void* stream, const cgn_token_rows* r, int32_
                                    float* coef, void* dlogits, int64_t ldd, void* workspace, int64_t workspace_bytes) {
     CGN_CHECK_ARG(base_ok(r) && T > 0 && r->M > 0 && r->M % (2 * (int64_t)T) == 0 && r->weight);
     CGN_CHECK_ARG(beta > 0.0 && label_smoothing >= 0.0 && label_smoothing < 0.5);
-    CGN_CHECK_ARG(ref_logp && loss && margin && seq_logp && (!dlogits || ldd >= r->V));
+    CGN_CHECK_ARG(ref_logp && loss && margin && seq_logp && (!dlogits || dest_ok(r, dlogits, ldd)));
     CGN_CHECK_ARG(workspace && (uintptr_t)workspace % 8 == 0);
     const int P = (int)(r->M / (2 * (int64_t)T));
     if (r->M * 24 + 16 > workspace_bytes) return CGN_ERR_WORKSPACE;

@@ -327,30 +327,34 @@ def _packed(t):
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _guard_capture(*leaves):
-    """Captured graphs and autograd. Autograd runs the accumulation into a leaf on the stream that was current when the
-    leaf entered the oldest of its graphs that are still alive; if that was outside of a stream capture, a backward pass
-    under capture pulls a foreign stream in and the runtime ends the process. Refused here: a forward pass under capture
-    whose leaves live in a graph that these forms built outside of it. What cannot be refused in time (the streams are tied
-    before any node runs) is a captured backward pass of a forward pass that was not captured: capture both, or use the
-    explicit forms in ops.py, which have no such limits."""
-    captured = torch.cuda.is_current_stream_capturing()
-    for t in leaves:
-        if t is None or not t.requires_grad or not t.is_leaf:
-            continue
-        seen = torch.autograd.graph.get_gradient_edge(t).node.metadata  # lives as long as a graph over the leaf does
-        if not captured:
-            seen["built outside of a capture"] = True
-        elif seen.get("built outside of a capture"):
+def _apply(fn, leaves, *args):
+    """fn.apply(*args), with an eye on captured graphs. Autograd runs the accumulation into a leaf on the stream that was
+    current when the leaf entered the oldest of its graphs that are still alive; if that was outside of a stream capture, a
+    backward pass under capture pulls a foreign stream in and the runtime ends the process. Refused here: a forward pass
+    under capture whose leaves live in a graph that these forms built outside of it. What cannot be refused in time (the
+    streams are tied before any node runs) is a captured backward pass of a forward pass that was not captured: capture
+    both, or use the explicit forms in ops.py, which have no such limits."""
+    if not torch.is_grad_enabled():
+        return fn.apply(*args)
+    leaves = [t for t in leaves if t is not None and t.requires_grad and t.is_leaf]
+    seen = lambda t: torch.autograd.graph.get_gradient_edge(t).node.metadata  # noqa: E731  (lives as a graph over t does)
+    if torch.cuda.is_current_stream_capturing():
+        if any([seen(t).get(_UNCAPTURED) for t in leaves]):
             raise RuntimeError("forward pass under stream capture while an autograd graph over the same parameters, built "
                                "outside of the capture, is alive: drop it (its outputs and losses) first")
+        return fn.apply(*args)
+    out = fn.apply(*args)
+    for t in leaves:
+        seen(t)[_UNCAPTURED] = True
+    return out
+
+
+_UNCAPTURED = "built outside of a capture"
 
 
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, W, b, eps):
-        need_cuda(x, "LayerNorm")
-        _guard_capture(x, W, b)
         x = _packed(x)
         y, mean, rstd = ops.layer_norm_fwd(x, W, b, eps)
         ctx.save_for_backward(x, W, mean, rstd)
@@ -382,7 +386,8 @@ class LayerNorm(nn.Module):
     def forward(self, x):
         if x.shape[-1] != self.features:
             raise ValueError("LayerNorm(%d) got rows of %d elements" % (self.features, x.shape[-1]))
-        return _LayerNormFn.apply(x, self.weight, self.bias, self.eps)
+        need_cuda(x, "LayerNorm")
+        return _apply(_LayerNormFn, (x, self.weight, self.bias), x, self.weight, self.bias, self.eps)
 
 
 # ------------------------------------------------------------------------------------------------------------------
@@ -392,8 +397,6 @@ class _PolicyLossFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, target, advantage, weight, old_logp, ref_logp, clip, kl_coef, inv_tau):
-        need_cuda(logits, "policy_loss")
-        _guard_capture(logits)
         logits = _packed(logits)
         loss, logp, stats, coef = ops.policy_loss(logits, target, advantage, weight, old_logp=old_logp, ref_logp=ref_logp,
                                                   clip=clip, kl_coef=kl_coef, inv_tau=inv_tau, save=True)
@@ -413,14 +416,13 @@ class _PolicyLossFn(torch.autograd.Function):
 def policy_loss(logits, target, advantage, weight=None, *, old_logp=None, ref_logp=None, clip=(0.2, 0.2), kl_coef=0.0,
                 inv_tau=1.0):
     """Clipped policy loss with a KL term (ops.policy_loss), differentiable in `logits` alone: (loss, logp)."""
-    return _PolicyLossFn.apply(logits, target, advantage, weight, old_logp, ref_logp, clip, kl_coef, inv_tau)
+    need_cuda(logits, "policy_loss")
+    return _apply(_PolicyLossFn, (logits,), logits, target, advantage, weight, old_logp, ref_logp, clip, kl_coef, inv_tau)
 
 
 class _PreferenceLossFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, target, weight, ref_logp, beta, label_smoothing, inv_tau):
-        need_cuda(logits, "preference_loss")
-        _guard_capture(logits)
         logits = _packed(logits)
         loss, margin, seq_logp, stats, coef = ops.preference_loss(logits, target, weight, ref_logp, beta=beta,
                                                                   label_smoothing=label_smoothing, inv_tau=inv_tau,
@@ -441,7 +443,8 @@ class _PreferenceLossFn(torch.autograd.Function):
 def preference_loss(logits, target, weight, ref_logp, *, beta, label_smoothing=0.0, inv_tau=1.0):
     """Preference loss over pairs of sentences (ops.preference_loss), differentiable in `logits` alone:
     (loss, margin, seq_logp)."""
-    return _PreferenceLossFn.apply(logits, target, weight, ref_logp, beta, label_smoothing, inv_tau)
+    need_cuda(logits, "preference_loss")
+    return _apply(_PreferenceLossFn, (logits,), logits, target, weight, ref_logp, beta, label_smoothing, inv_tau)
 
 
 # ------------------------------------------------------------------------------------------------------------------

@@ -1460,6 +1460,14 @@ def _rows_any(t, name):
     return b16, R, C_, ld
 
 
+def _own_or_apart(dst, ldd, src, lds, rows, cols, name):
+    """A destination is a matrix of its own or exactly the buffer of `src` (a row is read whole before it is written)."""
+    a, b, size = src.data_ptr(), dst.data_ptr(), src.element_size()
+    if rows and not (a == b and lds == ldd):
+        _req(a + ((rows - 1) * lds + cols) * size <= b or b + ((rows - 1) * ldd + cols) * size <= a,
+             "%s must be the source's own buffer or lie apart from it" % name)
+
+
 def _vector(t, n, name, dev):
     _chk_f32(t, name)
     if t.numel() != n or not t.is_contiguous() or t.device != dev:
@@ -1492,6 +1500,7 @@ def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5, out=None):
     else:
         _req(y.shape == x.shape and y.dtype == x.dtype and y.device == dev, "out must be like x")
         ldy = _rows_any(y, "out")[3]
+        _own_or_apart(y, ldy, x, ld, R, Cn, "out")
     mean, rstd = alloc((2, R), dev).unbind(0)
     _call("cgn_layer_norm_fwd", dev, x.data_ptr(), ld, R, Cn, b16, _addr(weight), _addr(bias), eps, y.data_ptr(), ldy,
           mean.data_ptr(), rstd.data_ptr())
@@ -1518,6 +1527,8 @@ def layer_norm_bwd(dy, x, weight, mean, rstd, dx=None, dweight=None, dbias=None,
     else:
         _req(dx.shape == x.shape and dx.dtype == x.dtype and dx.device == dev, "dx must be like x")
         lddx = _rows_any(dx, "dx")[3]
+        _own_or_apart(dx, lddx, x, ldx, R, Cn, "dx")
+        _own_or_apart(dx, lddx, dy, lddy, R, Cn, "dx")
     ws = None
     if params:
         _req(beta == 0.0 or (dbias is not None and (weight is None or dweight is not None)),
@@ -1577,10 +1588,7 @@ def _dlogits_dest(logits, ld, dlogits):
          "dlogits must be like logits, with unit column stride")
     ldd = dlogits.stride(0) if M > 1 else V
     _req(ldd >= V, "rows of dlogits must not overlap")
-    a, b, size = logits.data_ptr(), dlogits.data_ptr(), logits.element_size()
-    if M and not (a == b and ld == ldd):
-        _req(a + ((M - 1) * ld + V) * size <= b or b + ((M - 1) * ldd + V) * size <= a,
-             "dlogits must be the logits' own buffer or lie apart from it")
+    _own_or_apart(dlogits, ldd, logits, ld, M, V, "dlogits")
     return ldd
 
 

@@ -53,6 +53,7 @@ def test_wrappers_refuse_cpu_tensors():
 def test_layer_norm_refusals(host):
     x = torch.zeros(4, 8)
     v = torch.zeros(4)
+    buf = torch.zeros(64)
     bad = [
         lambda: ops.layer_norm_fwd(torch.zeros(4, 0)),
         lambda: ops.layer_norm_fwd(torch.zeros(1, ops.LAYER_NORM_MAX_COLS + 1)),
@@ -71,6 +72,11 @@ def test_layer_norm_refusals(host):
         lambda: ops.layer_norm_bwd(x, x, torch.zeros(8), v, v, dbias=torch.zeros(8), beta=1.0),
         lambda: ops.layer_norm_bwd(x, x, None, v, v, dbias=torch.zeros(8), params=False),
         lambda: ops.layer_norm_bwd(x, x, None, v, v, dx=torch.zeros(4, 7)),
+        # a destination that overlaps its source without being its buffer
+        lambda: ops.layer_norm_fwd(buf[:32].view(4, 8), out=buf[8:40].view(4, 8)),
+        lambda: ops.layer_norm_fwd(buf.view(4, 16)[:, :8], out=buf[:32].view(4, 8)),
+        lambda: ops.layer_norm_bwd(buf[:32].view(4, 8), x, None, v, v, dx=buf[4:36].view(4, 8)),
+        lambda: ops.layer_norm_bwd(x, buf[:32].view(4, 8), None, v, v, dx=buf[4:36].view(4, 8)),
     ]
     for f in bad:
         with pytest.raises(ValueError):
@@ -82,7 +88,9 @@ def test_layer_norm_refusals(host):
     assert not host
     ops.layer_norm_fwd(torch.zeros(4, 16)[:, :8], torch.zeros(8))
     ops.layer_norm_bwd(x, x, None, v, v, dx=False)
-    assert len(host) == 2
+    ops.layer_norm_fwd(x, out=x)
+    ops.layer_norm_bwd(x, torch.zeros(4, 8), None, v, v, dx=x)
+    assert len(host) == 4
 
 
 def test_token_loss_refusals(host):
@@ -206,7 +214,7 @@ def test_entry_points_refuse_bad_arguments():
         return C.byref(r)
 
     for k in (dict(M=-1), dict(V=0), dict(ld=7), dict(inv_tau=0.0), dict(inv_tau=float("nan")), dict(logits=None),
-              dict(target=None), dict(M=1 << 31)):
+              dict(target=None), dict(M=1 << 31), dict(logits=4098), dict(logits=4097, bf16=1)):
         assert lib.cgn_token_logp(None, rows(**k), P, P) == BAD, k
         assert lib.cgn_token_logp_bwd(None, rows(**k), P, P, None, P, 8) == BAD, k
     assert lib.cgn_token_logp(None, rows(), None, P) == BAD

@@ -380,6 +380,9 @@ def test_masked_rows_strides_and_bad_values(dev, V, extra, shift, dtype):
     loss, logp = ops.policy_loss(x0, t3, A, w, old_logp=old, dlogits=d)
     assert loss.isnan().all() and logp[2].isnan() and d[2].isnan().all()
     assert torch.isfinite(d[[0, 1, 3, 4, 5, 6, 7]].float()).all() and torch.isfinite(logp[[0, 5]]).all()
+    stats = ops.token_logp(x0, t3, w)[1]
+    d = ops.token_logp_bwd(x0, t3, stats, torch.ones(M, device=dev), weight=w)
+    assert d[2].isnan().all() and torch.isfinite(d[[0, 5]].float()).all()
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -563,6 +566,21 @@ def test_long_offsets(dev):
     ops.token_logp_bwd(x, target, stats, coef, weight=w, dlogits=d)
     check_dlogits(d[-3:], want["d"], want["d_tol"], "dlogits, second pass")
     assert not d[:-3].any()
+
+
+def test_more_rows_than_a_grid_holds(dev):
+    """2^31 threads are the most of one launch: the rows behind that take another one."""
+    M, V = (1 << 23) + 5, 3
+    x = torch.randn(M, V, device=dev, generator=gen(6))
+    t = torch.randint(0, V, (M,), device=dev, generator=gen(7))
+    A = torch.randn(M, device=dev, generator=gen(8))
+    w = (torch.rand(M, device=dev, generator=gen(9)) < 0.9).float() / M
+    d = torch.empty_like(x)
+    loss, logp = ops.policy_loss(x, t, A, w, dlogits=d)
+    want = policy_ref(x, t, A, w, None, None, 0.2, 0.2, 0.0, 1.0)
+    close(logp, want["logp"], want["band"], "logp")
+    assert abs(float(loss) - float(want["loss"])) <= want["loss_tol"] + 2 * U * abs(float(want["loss"]))
+    check_dlogits(d, want["d"], want["d_tol"], "dlogits")
 
 
 # ---------------------------------------------------------------------------------------------------------------------
@@ -865,6 +883,14 @@ def test_captured_modules(dev):
         with pytest.raises(RuntimeError, match="alive"):
             with torch.cuda.graph(graph, stream=side):
                 ln(x)
+        with torch.no_grad():  # no backward pass can follow: taken
+            free = torch.cuda.CUDAGraph()
+            with ops.capture_without_gc():
+                with torch.cuda.graph(free, stream=side):
+                    y = ln(x)
+            free.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, alive)
         del alive
         torch.cuda.synchronize()
         static = x.clone()
