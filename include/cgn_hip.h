@@ -677,18 +677,20 @@ typedef struct cgn_grad_tensor {
 /* Bytes of workspace that the two calls below need for this list (host call; 8-byte aligned). clip != 0: the list is
  * for cgn_clip_grads, and refused as that refuses it. */
 int cgn_grad_norm_workspace(const cgn_grad_tensor* t, int32_t n, int32_t clip, int64_t* bytes);
-/* norm[0] = |scale| * sqrt(sum g^2) over all tensors (max_abs != 0: |scale| * max |g|); coef (nullable)
- * [0] = min(1, max_norm / (norm + 1e-6)). NaN gradients give NaN (csrc/gradnorm.hip). */
-int cgn_grad_norm(void* stream, const cgn_grad_tensor* t, int32_t n, int32_t max_abs, double scale, double max_norm,
-                  float* norm, float* coef, void* workspace, int64_t workspace_bytes);
+/* norm[0] = |scale| * sqrt(sum g^2) over all tensors (max_abs != 0: |scale| * max |g|). NaN gradients give NaN
+ * (csrc/gradnorm.hip). */
+int cgn_grad_norm(void* stream, const cgn_grad_tensor* t, int32_t n, int32_t max_abs, double scale, float* norm,
+                  void* workspace, int64_t workspace_bytes);
 /* The same norm, and out = g * scale * min(1, max_norm / (norm + 1e-6)) for every tensor. out may be g; apart from that
  * no two ranges of memory (first to last element) of the list may overlap: CGN_ERR_INVALID_ARG. */
 int cgn_clip_grads(void* stream, const cgn_grad_tensor* t, int32_t n, int32_t max_abs, double scale, double max_norm,
                    float* norm, void* workspace, int64_t workspace_bytes);
-/* cgn_adam_f32 with the gradients read as g * grad_scale * clip_coef[0] (device): the update behind cgn_grad_norm. */
+/* cgn_adam_f32 with the gradient clipped on the way in: norm[0] = |grad_scale| * sqrt(sum g^2), and g is read as
+ * g * grad_scale * min(1, max_norm / (norm + 1e-6)); g itself stays as it is. n >= 1. */
+#define CGN_ADAM_CLIP_WORKSPACE 8256 /* bytes, 8-byte aligned */
 int cgn_adam_clipped_f32(void* stream, float* p, const float* g, float* m, float* v, int64_t n, float lr, float beta1,
                          float beta2, float eps, int32_t step, const int32_t* dyn_step, float grad_scale,
-                         const float* clip_coef);
+                         double max_norm, float* norm, void* workspace, int64_t workspace_bytes);
 
 #ifdef __cplusplus
 }

@@ -69,3 +69,12 @@ __device__ __forceinline__ float block_max(float v, float* red) {
     for (int i = 1; i < NT / 64; ++i) t = fmaxf(t, red[i]);
     return t;
 }
+
+// gradnorm.hip, for the clipped Adam update in pointwise.hip
+int cgn_arena_norm(void* stream, const float* g, int64_t n, double scale, double max_norm, float* norm, float* coef,
+                   double* part, int* parts);
+// The clipping factor min(1, max_norm / (norm + 1e-6)); a NaN norm stays one.
+__device__ __forceinline__ float cgn_clip_factor(double norm, double max_norm) {
+    const double c = max_norm / (norm + 1e-6);
+    return c > 1.0 ? 1.f : (float)c;
+}

@@ -15,6 +15,7 @@ using namespace cgn_rows;
 
 constexpr int GN_NT = 512;
 constexpr int GN_MAX = 72;         // tensors per launch: their descriptions travel as kernel arguments (below 4 KB)
+constexpr int GN_FEW = 8;
 constexpr int GN_BLOCKS = 1024;    // partials of a long list of elements: four workgroups per CU
 constexpr int64_t GN_CHUNK = 4096;  // elements a workgroup takes at least
 
@@ -25,9 +26,10 @@ struct Seg {
     int rows, bf16;
 };
 
+template <int N>
 struct Segs {
-    Seg seg[GN_MAX];
-    int first[GN_MAX + 1];  // first workgroup of every tensor
+    Seg seg[N];
+    int first[N + 1];  // first workgroup of every tensor
     int n;
     bool stream;  // the list is past the caches' size (rows.h)
     long chunk;
@@ -39,7 +41,8 @@ struct Span {
     long c0, c1;
 };
 
-__device__ __forceinline__ Span span_of(const Segs& a, int b) {
+template <int N>
+__device__ __forceinline__ Span span_of(const Segs<N>& a, int b) {
     int lo = 0, hi = a.n - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -124,8 +127,8 @@ __device__ __forceinline__ double part_of(const Seg& s, const Span& p) {
     return t;
 }
 
-template <bool MAX>
-__global__ __launch_bounds__(GN_NT) void norm_part_kernel(const Segs a, double* __restrict__ part) {
+template <bool MAX, int N>
+__global__ __launch_bounds__(GN_NT) void norm_part_kernel(const Segs<N> a, double* __restrict__ part) {
     __shared__ double red[GN_NT / 64];
     const Span p = span_of(a, blockIdx.x);
     const Seg& s = a.seg[p.t];
@@ -142,9 +145,8 @@ __device__ __forceinline__ void total_of(const double* part, int n, double scale
     for (int i = threadIdx.x; i < n; i += GN_NT) v = join<MAX>(v, part[i]);
     v = block_join<MAX>(v, red);
     const double nrm = (MAX ? v : sqrt(v)) * fabs(scale);
-    const double c = max_norm / (nrm + 1e-6);
     *norm = (float)nrm;
-    *coef = c > 1.0 ? 1.f : (float)c;
+    *coef = cgn_clip_factor(nrm, max_norm);
 }
 
 template <bool MAX>
@@ -191,8 +193,8 @@ __device__ __forceinline__ void scale_part(const Seg& s, const Span& p, float f,
 
 // Every workgroup joins the partials itself (a few KB from the L2): one launch less than a kernel for it alone. The spans
 // are walked backwards: what the norm's pass read last is still in the 256 MB cache.
-template <bool MAX>
-__global__ __launch_bounds__(GN_NT) void clip_kernel(const Segs a, const double* __restrict__ part, int nparts,
+template <bool MAX, int N>
+__global__ __launch_bounds__(GN_NT) void clip_kernel(const Segs<N> a, const double* __restrict__ part, int nparts,
                                                      double scale, double max_norm, float* __restrict__ norm) {
     __shared__ double red[GN_NT / 64];
     float v, c;
@@ -261,12 +263,13 @@ int64_t blocks_of(const cgn_grad_tensor& t, int64_t chunk) {
 }
 
 // Fills one launch from tensor i on; returns the tensor behind it.
-int pack(const cgn_grad_tensor* t, int n, int i, int64_t chunk, Segs* a, int64_t* blocks) {
+template <int N>
+int pack(const cgn_grad_tensor* t, int n, int i, int64_t chunk, Segs<N>* a, int64_t* blocks) {
     a->n = 0;
     a->chunk = chunk;
     a->stream = chunk * GN_BLOCKS * 4 >= STREAM_BYTES;
     *blocks = 0;
-    for (; i < n && a->n < GN_MAX; ++i) {
+    for (; i < n && a->n < N; ++i) {
         const int64_t b = blocks_of(t[i], chunk);
         if (b == 0) continue;
         a->seg[a->n] = Seg{t[i].g, t[i].out, (long)t[i].cols, (long)t[i].ld, (long)t[i].ldo, (int)t[i].rows,
@@ -285,20 +288,26 @@ int64_t parts_of(const cgn_grad_tensor* t, int n) {
     return parts;
 }
 
-template <bool MAX>
-int norm_parts(hipStream_t s, const cgn_grad_tensor* t, int n, double* part) {
+template <bool MAX, int N>
+int norm_parts_in(hipStream_t s, const cgn_grad_tensor* t, int n, double* part) {
     const int64_t chunk = chunk_of(t, n);
     int64_t done = 0;
     for (int i = 0; i < n;) {
-        Segs a;
+        Segs<N> a;
         int64_t blocks;
         i = pack(t, n, i, chunk, &a, &blocks);
         if (blocks == 0) continue;
-        hipLaunchKernelGGL(norm_part_kernel<MAX>, dim3((unsigned)blocks), dim3(GN_NT), 0, s, a, part + done);
+        hipLaunchKernelGGL((norm_part_kernel<MAX, N>), dim3((unsigned)blocks), dim3(GN_NT), 0, s, a, part + done);
         CGN_LAUNCH_CHECK();
         done += blocks;
     }
     return CGN_OK;
+}
+
+// (a short list's description is a tenth of the kernel arguments that a full one takes)
+template <bool MAX>
+int norm_parts(hipStream_t s, const cgn_grad_tensor* t, int n, double* part) {
+    return n <= GN_FEW ? norm_parts_in<MAX, GN_FEW>(s, t, n, part) : norm_parts_in<MAX, GN_MAX>(s, t, n, part);
 }
 
 template <bool MAX>
@@ -311,19 +320,16 @@ int run_norm(hipStream_t s, const cgn_grad_tensor* t, int n, double scale, doubl
     return CGN_OK;
 }
 
-template <bool MAX>
-int run_clip(hipStream_t s, const cgn_grad_tensor* t, int n, double scale, double max_norm, float* norm, double* part,
-             int parts) {
-    if (parts == 0) return run_norm<MAX>(s, t, n, scale, max_norm, norm, nullptr, part, 0);
-    const int rc = norm_parts<MAX>(s, t, n, part);
-    if (rc != CGN_OK) return rc;
+template <bool MAX, int N>
+int clip_in(hipStream_t s, const cgn_grad_tensor* t, int n, double scale, double max_norm, float* norm,
+            const double* part, int parts) {
     const int64_t chunk = chunk_of(t, n);
     for (int i = 0; i < n;) {
-        Segs a;
+        Segs<N> a;
         int64_t blocks;
         i = pack(t, n, i, chunk, &a, &blocks);
         if (blocks == 0) continue;
-        hipLaunchKernelGGL(clip_kernel<MAX>, dim3((unsigned)blocks), dim3(GN_NT), 0, s, a, part, parts, scale, max_norm,
+        hipLaunchKernelGGL((clip_kernel<MAX, N>), dim3((unsigned)blocks), dim3(GN_NT), 0, s, a, part, parts, scale, max_norm,
                            norm);
         CGN_LAUNCH_CHECK();
         norm = nullptr;  // written once
@@ -331,7 +337,26 @@ int run_clip(hipStream_t s, const cgn_grad_tensor* t, int n, double scale, doubl
     return CGN_OK;
 }
 
+template <bool MAX>
+int run_clip(hipStream_t s, const cgn_grad_tensor* t, int n, double scale, double max_norm, float* norm, double* part,
+             int parts) {
+    if (parts == 0) return run_norm<MAX>(s, t, n, scale, max_norm, norm, nullptr, part, 0);
+    const int rc = norm_parts<MAX>(s, t, n, part);
+    if (rc != CGN_OK) return rc;
+    return n <= GN_FEW ? clip_in<MAX, GN_FEW>(s, t, n, scale, max_norm, norm, part, parts)
+                       : clip_in<MAX, GN_MAX>(s, t, n, scale, max_norm, norm, part, parts);
+}
+
 }  // namespace
+
+// One flat fp32 arena: the partials of its sum of squares in part[0 .. *parts), and with `coef` the norm and the factor too.
+int cgn_arena_norm(void* stream, const float* g, int64_t n, double scale, double max_norm, float* norm, float* coef,
+                   double* part, int* parts) {
+    const cgn_grad_tensor t = {g, nullptr, 1, n, 0, 0, 0};
+    *parts = (int)parts_of(&t, 1);
+    hipStream_t s = (hipStream_t)stream;
+    return coef ? run_norm<false>(s, &t, 1, scale, max_norm, norm, coef, part, *parts) : norm_parts<false>(s, &t, 1, part);
+}
 
 extern "C" int cgn_grad_norm_workspace(const cgn_grad_tensor* t, int32_t n, int32_t clip, int64_t* bytes) {
     CGN_CHECK_ARG(n >= 0 && bytes && (n == 0 || t) && segs_ok(t, n, clip != 0) && (!clip || apart(t, n)));
@@ -341,18 +366,18 @@ extern "C" int cgn_grad_norm_workspace(const cgn_grad_tensor* t, int32_t n, int3
     return CGN_OK;
 }
 
-extern "C" int cgn_grad_norm(void* stream, const cgn_grad_tensor* t, int32_t n, int32_t max_abs, double scale,
-                             double max_norm, float* norm, float* coef, void* workspace, int64_t workspace_bytes) {
+extern "C" int cgn_grad_norm(void* stream, const cgn_grad_tensor* t, int32_t n, int32_t max_abs, double scale, float* norm,
+                             void* workspace, int64_t workspace_bytes) {
     int64_t need;
     const int rc = cgn_grad_norm_workspace(t, n, 0, &need);
     if (rc != CGN_OK) return rc;
-    CGN_CHECK_ARG(norm && max_norm >= 0.0 && workspace && (uintptr_t)workspace % 8 == 0);
+    CGN_CHECK_ARG(norm && workspace && (uintptr_t)workspace % 8 == 0);
     if (need > workspace_bytes) return CGN_ERR_WORKSPACE;
     const int parts = (int)((need - 8) / 8);
     hipStream_t s = (hipStream_t)stream;
     double* part = (double*)workspace;
-    return max_abs ? run_norm<true>(s, t, n, scale, max_norm, norm, coef, part, parts)
-                   : run_norm<false>(s, t, n, scale, max_norm, norm, coef, part, parts);
+    return max_abs ? run_norm<true>(s, t, n, scale, 0.0, norm, nullptr, part, parts)
+                   : run_norm<false>(s, t, n, scale, 0.0, norm, nullptr, part, parts);
 }
 
 extern "C" int cgn_clip_grads(void* stream, const cgn_grad_tensor* t, int32_t n, int32_t max_abs, double scale,

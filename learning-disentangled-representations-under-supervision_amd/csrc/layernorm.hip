@@ -306,7 +306,7 @@ __global__ __launch_bounds__(LNF_NT) void layer_norm_params_kernel(const float* 
 }
 
 constexpr int LN_MAX_C = 8192;    // widest row that the groups below hold in registers
-constexpr int LN_ALONE = 4;       // a backward pass of that many workgroups' rows is left to one
+constexpr int LN_ALONE = 8;       // a backward pass of that many workgroups' rows is left to one
 constexpr int LN_FWD_NB = 8192;   // workgroups of a forward pass at most: each with many rows behind one read of w and b
 
 template <typename T, int NT, int G, int NV>

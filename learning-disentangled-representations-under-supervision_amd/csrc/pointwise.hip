@@ -230,13 +230,41 @@ __global__ __launch_bounds__(PW_NT) void rowdot_kernel(const float* __restrict__
     }
 }
 
+// How an Adam update clips its gradient: not at all, by a factor on the device, or by the partial sums of squares, which
+// every workgroup then joins itself (few of them: one launch less).
+struct AdamClip {
+    const float* coef;
+    const double* part;
+    int nparts;
+    float* norm;
+    double scale, max_norm;
+};
+
+__device__ __forceinline__ float adam_clip(const AdamClip& a) {
+    if (a.coef) return a.coef[0];
+    if (!a.part) return 1.f;
+    __shared__ double red[PW_NT / 64];
+    double s = 0.0;
+    for (int i = threadIdx.x; i < a.nparts; i += PW_NT) s += a.part[i];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = 0.0;
+#pragma unroll
+    for (int w = 0; w < PW_NT / 64; ++w) s += red[w];
+    const double norm = sqrt(s) * fabs(a.scale);
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.norm[0] = (float)norm;
+    return cgn_clip_factor(norm, a.max_norm);
+}
+
 // ---- Adam (torch.optim.Adam defaults: bias-corrected, no weight decay, no amsgrad; model/cgn.py:267,1046-1047) -----
 __global__ __launch_bounds__(PW_NT) void adam_kernel(float* __restrict__ p, const float* __restrict__ g,
                                                      float* __restrict__ m, float* __restrict__ v, long n, float lr,
                                                      float b1, float b2, float eps, float bc1, float bc2_sqrt,
                                                      const int* __restrict__ dyn_step, float grad_scale,
-                                                     const float* __restrict__ clip_coef) {
-    if (clip_coef) grad_scale *= clip_coef[0];
+                                                     const AdamClip clip) {
+    grad_scale *= adam_clip(clip);
     if (dyn_step) {  // device-resident step count: same double-precision bias corrections as the host path
         const double t = (double)dyn_step[0];
         bc1 = (float)(1.0 - pow((double)b1, t));
@@ -280,8 +308,8 @@ __global__ __launch_bounds__(PW_NT) void adam_vec4_kernel(float* __restrict__ p,
                                                           float* __restrict__ m, float* __restrict__ v, long n, float lr,
                                                           float b1, float b2, float eps, float bc1, float bc2_sqrt,
                                                           const int* __restrict__ dyn_step, float grad_scale,
-                                                          const float* __restrict__ clip_coef) {
-    if (clip_coef) grad_scale *= clip_coef[0];
+                                                          const AdamClip clip) {
+    grad_scale *= adam_clip(clip);
     if (dyn_step) {
         const double t = (double)dyn_step[0];
         bc1 = (float)(1.0 - pow((double)b1, t));
@@ -672,7 +700,7 @@ extern "C" int cgn_rowdot_f32(void* stream, const float* a, int64_t lda, const f
 }
 
 static int adam(void* stream, float* p, const float* g, float* m, float* v, int64_t n, float lr, float beta1, float beta2,
-                float eps, int32_t step, const int32_t* dyn_step, float grad_scale, const float* clip_coef) {
+                float eps, int32_t step, const int32_t* dyn_step, float grad_scale, const AdamClip& clip) {
     CGN_CHECK_ARG(n >= 0 && (dyn_step || step >= 1));
     if (n == 0) return CGN_OK;
     CGN_CHECK_ARG(p && g && m && v);
@@ -683,27 +711,45 @@ static int adam(void* stream, float* p, const float* g, float* m, float* v, int6
     const bool vec = (((uintptr_t)p | (uintptr_t)g | (uintptr_t)m | (uintptr_t)v) % 16 == 0) && n >= 4;
     if (vec && n >= (32 << 20))
         hipLaunchKernelGGL(adam_vec4_kernel<true>, dim3(pw_blocks(n / 4, PW_NT, 65536)), dim3(PW_NT), 0, S_(stream), p, g, m,
-                           v, (long)n, lr, beta1, beta2, eps, (float)bc1, (float)sqrt(bc2), dyn_step, grad_scale, clip_coef);
+                           v, (long)n, lr, beta1, beta2, eps, (float)bc1, (float)sqrt(bc2), dyn_step, grad_scale, clip);
     else if (vec)
         hipLaunchKernelGGL(adam_vec4_kernel<false>, dim3(pw_blocks(n / 4, PW_NT, 8192)), dim3(PW_NT), 0, S_(stream), p, g, m, v,
-                           (long)n, lr, beta1, beta2, eps, (float)bc1, (float)sqrt(bc2), dyn_step, grad_scale, clip_coef);
+                           (long)n, lr, beta1, beta2, eps, (float)bc1, (float)sqrt(bc2), dyn_step, grad_scale, clip);
     else
         hipLaunchKernelGGL(adam_kernel, dim3(pw_blocks(n, PW_NT, 8192)), dim3(PW_NT), 0, S_(stream), p, g, m, v, (long)n,
-                           lr, beta1, beta2, eps, (float)bc1, (float)sqrt(bc2), dyn_step, grad_scale, clip_coef);
+                           lr, beta1, beta2, eps, (float)bc1, (float)sqrt(bc2), dyn_step, grad_scale, clip);
     CGN_LAUNCH_CHECK();
     return CGN_OK;
 }
 
 extern "C" int cgn_adam_f32(void* stream, float* p, const float* g, float* m, float* v, int64_t n, float lr, float beta1,
                             float beta2, float eps, int32_t step, const int32_t* dyn_step, float grad_scale) {
-    return adam(stream, p, g, m, v, n, lr, beta1, beta2, eps, step, dyn_step, grad_scale, nullptr);
+    return adam(stream, p, g, m, v, n, lr, beta1, beta2, eps, step, dyn_step, grad_scale, AdamClip{});
 }
 
 extern "C" int cgn_adam_clipped_f32(void* stream, float* p, const float* g, float* m, float* v, int64_t n, float lr,
                                     float beta1, float beta2, float eps, int32_t step, const int32_t* dyn_step,
-                                    float grad_scale, const float* clip_coef) {
-    CGN_CHECK_ARG(clip_coef);
-    return adam(stream, p, g, m, v, n, lr, beta1, beta2, eps, step, dyn_step, grad_scale, clip_coef);
+                                    float grad_scale, double max_norm, float* norm, void* workspace,
+                                    int64_t workspace_bytes) {
+    CGN_CHECK_ARG(n > 0 && p && g && m && v && (dyn_step || step >= 1) && max_norm >= 0.0 && norm);
+    CGN_CHECK_ARG(workspace && (uintptr_t)workspace % 8 == 0);
+    if (workspace_bytes < CGN_ADAM_CLIP_WORKSPACE) return CGN_ERR_WORKSPACE;
+    AdamClip clip = {};
+    clip.norm = norm;
+    clip.scale = (double)grad_scale;
+    clip.max_norm = max_norm;
+    double* part = (double*)workspace;
+    float* coef = (float*)(part + 1024);  // (behind the most partials that a list of one tensor leaves)
+    // up to 256 partials (a million elements) every workgroup of the update joins them, 2 KB from the L2; above, a kernel of
+    // one workgroup does (5 us with its launch, of 20 and more)
+    const bool few = n <= (1 << 20);
+    const int rc = cgn_arena_norm(stream, g, n, (double)grad_scale, max_norm, norm, few ? nullptr : coef, part, &clip.nparts);
+    if (rc != CGN_OK) return rc;
+    if (few)
+        clip.part = part;
+    else
+        clip.coef = coef;
+    return adam(stream, p, g, m, v, n, lr, beta1, beta2, eps, step, dyn_step, grad_scale, clip);
 }
 
 extern "C" int cgn_incr_i32(void* stream, int32_t* counter) {

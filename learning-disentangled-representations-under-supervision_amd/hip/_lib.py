@@ -122,6 +122,8 @@ class GradTensor(C.Structure):
                 ("bf16", c_i64)]
 
 
+ADAM_CLIP_WORKSPACE = 8256  # bytes
+
 ACT_RELU = 0
 ACT_TANH = 1
 
@@ -208,10 +210,10 @@ PROTOTYPES = {
     "cgn_preference_loss": (c_i32, [c_ptr, C.POINTER(TokenRows), c_i32, c_ptr, c_f64, c_f64, c_ptr, c_ptr, c_ptr, c_ptr,
                                     c_ptr, c_ptr, c_i64, c_ptr, c_i64]),
     "cgn_grad_norm_workspace": (c_i32, [c_ptr, c_i32, c_i32, C.POINTER(c_i64)]),
-    "cgn_grad_norm": (c_i32, [c_ptr, c_ptr, c_i32, c_i32, c_f64, c_f64, c_ptr, c_ptr, c_ptr, c_i64]),
+    "cgn_grad_norm": (c_i32, [c_ptr, c_ptr, c_i32, c_i32, c_f64, c_ptr, c_ptr, c_i64]),
     "cgn_clip_grads": (c_i32, [c_ptr, c_ptr, c_i32, c_i32, c_f64, c_f64, c_ptr, c_ptr, c_i64]),
     "cgn_adam_clipped_f32": (c_i32, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_f32, c_f32, c_f32, c_f32, c_i32, c_ptr,
-                                     c_f32, c_ptr]),
+                                     c_f32, c_f64, c_ptr, c_ptr, c_i64]),
     "cgn_cast_bf16_f32": (c_i32, [c_ptr, c_ptr, Axis, c_i32, c_i32, c_ptr, c_i64, c_i32]),
 }
 

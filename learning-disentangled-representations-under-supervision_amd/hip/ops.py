@@ -949,9 +949,12 @@ def adam(p, g, m, v, lr, step, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0,
         _call("cgn_adam_f32", p.device, _ptr(p), _ptr(g), _ptr(m), _ptr(v), n, lr, beta1, beta2, eps, int(step),
               _ptr(dyn_step), grad_scale)
         return None
-    norm, coef = _grad_norm([g], 2.0, grad_scale, max_norm)
-    _call("cgn_adam_clipped_f32", p.device, _ptr(p), _ptr(g), _ptr(m), _ptr(v), n, lr, beta1, beta2, eps, int(step),
-          _ptr(dyn_step), grad_scale, _ptr(coef))
+    max_norm = float(max_norm)
+    _req(max_norm >= 0.0 and n > 0, "max_norm must not be negative, and there must be something to clip")
+    dev = p.device
+    norm, ws = alloc((1,), dev), alloc((_lib.ADAM_CLIP_WORKSPACE // 8,), dev, torch.float64)
+    _call("cgn_adam_clipped_f32", dev, p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), n, lr, beta1, beta2, eps,
+          int(step), _addr(dyn_step), grad_scale, max_norm, norm.data_ptr(), ws.data_ptr(), ws.numel() * 8)
     return norm
 
 
@@ -1753,23 +1756,18 @@ def _norm_workspace(table, n, dev, clip):
     return alloc((nb.value // 8,), dev, torch.float64)
 
 
-def _grad_norm(grads, norm_type, grad_scale, max_norm):
-    kind = _norm_kind(norm_type)
-    max_norm = float(max_norm)
-    _req(max_norm >= 0.0, "max_norm must not be negative")
-    table, n, dev = _grad_table(grads, None)
-    ws = _norm_workspace(table, n, dev, 0)
-    norm, coef = alloc((2, 1), dev).unbind(0)
-    _call("cgn_grad_norm", dev, table.buffer_info()[0], n, kind, float(grad_scale), max_norm, norm.data_ptr(),
-          coef.data_ptr(), ws.data_ptr(), ws.numel() * 8)
-    return norm, coef
-
-
 def grad_norm(grads, norm_type=2.0, grad_scale=1.0):
     """Norm of all elements of a list of tensors (float32 / bfloat16, mixed) taken as one vector, times |grad_scale|:
     device tensor [1]. norm_type 2 or inf. A tensor is one piece of memory or a matrix with a row stride. The squares are
     summed in 64 bits; nothing is read back to the host."""
-    return _grad_norm(_grad_list(grads), norm_type, grad_scale, 0.0)[0]
+    grads = _grad_list(grads)
+    kind = _norm_kind(norm_type)
+    table, n, dev = _grad_table(grads, None)
+    ws = _norm_workspace(table, n, dev, 0)
+    norm = alloc((1,), dev)
+    _call("cgn_grad_norm", dev, table.buffer_info()[0], n, kind, float(grad_scale), norm.data_ptr(), ws.data_ptr(),
+          ws.numel() * 8)
+    return norm
 
 
 def clip_grad_norm(grads, max_norm, norm_type=2.0, out=None, grad_scale=1.0):

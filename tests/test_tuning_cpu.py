@@ -245,8 +245,8 @@ def test_entry_points_refuse_bad_arguments():
         assert lib.cgn_grad_norm_workspace(tb, n, 0, C.byref(nb)) == BAD, t
     tb, n = table((4096, 4096, 1, 10 ** 9, 0, 0, 0), (4096, 4096, 300, 825, 828, 828, 0), (0, 0, 1, 0, 0, 0, 0))
     assert lib.cgn_grad_norm_workspace(tb, n, 0, C.byref(nb)) == _lib.CGN_OK and 8 * 1000 < nb.value < 8 * 2000
-    assert lib.cgn_grad_norm(None, tb, n, 0, 1.0, 1.0, P, P, P, 8) == _lib.CGN_ERR_WORKSPACE
-    assert lib.cgn_grad_norm(None, tb, n, 0, 1.0, -1.0, P, P, P, nb.value) == BAD
+    assert lib.cgn_grad_norm(None, tb, n, 0, 1.0, P, P, 8) == _lib.CGN_ERR_WORKSPACE
+    assert lib.cgn_grad_norm(None, tb, n, 0, 1.0, None, P, nb.value) == BAD
     assert lib.cgn_clip_grads(None, tb, n, 0, 1.0, float("nan"), P, P, nb.value) == BAD
     assert lib.cgn_clip_grads(None, tb, n, 0, 1.0, 1.0, None, P, nb.value) == BAD
     tb, n = table((4096, 0, 1, 4, 0, 0, 0))
@@ -259,7 +259,15 @@ def test_entry_points_refuse_bad_arguments():
     assert lib.cgn_grad_norm_workspace(tb, n, 1, C.byref(nb)) == _lib.CGN_OK
     tb, n = table((4096, 4108, 1, 4, 0, 0, 0))
     assert lib.cgn_grad_norm_workspace(tb, n, 1, C.byref(nb)) == BAD
-    assert lib.cgn_adam_clipped_f32(None, P, P, P, P, 4, 1e-3, 0.9, 0.999, 1e-8, 1, None, 1.0, None) == BAD
+    ad = lambda **k: lib.cgn_adam_clipped_f32(None, P, k.get("g", P), P, P, k.get("n", 4), 1e-3, 0.9, 0.999, 1e-8,  # noqa: E731
+                                              k.get("step", 1), None, 1.0, k.get("max_norm", 1.0), k.get("norm", P),
+                                              k.get("ws", P), k.get("bytes", _lib.ADAM_CLIP_WORKSPACE))
+    for k in (dict(g=None), dict(n=0), dict(n=-1), dict(step=0), dict(max_norm=-1.0), dict(max_norm=float("nan")),
+              dict(norm=None), dict(ws=None), dict(ws=C.c_void_p(4100))):
+        assert ad(**k) == BAD, k
+    assert ad(bytes=_lib.ADAM_CLIP_WORKSPACE - 1) == _lib.CGN_ERR_WORKSPACE
+    header = open(os.path.join(ROOT, "include", "cgn_hip.h")).read()
+    assert "#define CGN_ADAM_CLIP_WORKSPACE %d " % _lib.ADAM_CLIP_WORKSPACE in header
 
 
 def test_struct_layouts_match_header(tmp_path):

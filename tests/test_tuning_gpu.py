@@ -700,7 +700,7 @@ def test_clip_parameters(dev):
     assert float(hnn.clip_grad_norm_([unused], 1.0)) == 0.0
 
 
-@pytest.mark.parametrize("n", [1, 5, 4099, 300001])
+@pytest.mark.parametrize("n", [1, 5, 4099, 300001, 1 << 20, (1 << 20) + 1, 33554433])
 def test_adam_clipped(dev, n):
     g = gen(n)
     mk = lambda s=1.0: s * torch.randn(n, device=dev, generator=g)  # noqa: E731
