@@ -9,14 +9,15 @@ namespace {
 
 using namespace cgn_rows;
 
-// Sums over the row's group: inside the wave with shuffles, over a whole workgroup through LDS.
+// Sums over the row's group: inside the wave with shuffles, over a whole workgroup through LDS. Calls in a row alternate
+// between two buffers `red`, so that one barrier each is enough: whoever writes a buffer again has passed the barrier of the
+// call in between, behind which nobody reads it any more.
 template <int NT, int G, int K>
 __device__ __forceinline__ void row_sums(float (&s)[K], float* red) {
     static_assert(G <= 64 || G == NT, "a group is part of a wave or the whole workgroup");
 #pragma unroll
     for (int k = 0; k < K; ++k) s[k] = group_sum<(G < 64 ? G : 64)>(s[k]);
     if constexpr (G > 64) {
-        __syncthreads();  // (the previous call's readers are done)
         if ((threadIdx.x & 63) == 0) {
 #pragma unroll
             for (int k = 0; k < K; ++k) red[(threadIdx.x >> 6) * K + k] = s[k];
@@ -86,7 +87,7 @@ __global__ __launch_bounds__(NT) void layer_norm_fwd_kernel(const T* x, long ldx
                                                             float eps, T* y, long ldy, float* __restrict__ mean,
                                                             float* __restrict__ rstd, bool stream) {
     constexpr int E = Piece<T>::E;
-    __shared__ float red[NT / 64 * 2];
+    __shared__ float red[2][NT / 64 * 2];
     const int lane = threadIdx.x % G;
     const int nfull = C / E, rem = C % E;
     const float inv_c = 1.f / (float)C;
@@ -101,7 +102,7 @@ __global__ __launch_bounds__(NT) void layer_norm_fwd_kernel(const T* x, long ldx
         for (int j = 0; j < NV; ++j)
 #pragma unroll
             for (int e = 0; e < E; ++e) s1[0] += row.q[j].get(e);
-        row_sums<NT, G, 1>(s1, red);
+        row_sums<NT, G, 1>(s1, red[0]);
         const float mu = s1[0] * inv_c;
         float s2[2] = {0.f, 0.f};
 #pragma unroll
@@ -119,7 +120,7 @@ __global__ __launch_bounds__(NT) void layer_norm_fwd_kernel(const T* x, long ldx
             s2[0] += d;
             s2[1] += d * d;
         }
-        row_sums<NT, G, 2>(s2, red);
+        row_sums<NT, G, 2>(s2, red[1]);
         const float off = s2[0] * inv_c;
         const float v = s2[1] * inv_c - off * off;
         const float rs = 1.f / sqrtf((v < 0.f ? 0.f : v) + eps);  // (a NaN stays one)
@@ -156,7 +157,8 @@ __global__ __launch_bounds__(NT) void layer_norm_bwd_kernel(const T* dy, long ld
                                                             bool stream) {
     constexpr int E = Piece<T>::E;
     constexpr int GROUPS = NT / G;
-    __shared__ float red[NT / 64 * 3];
+    __shared__ float red[2][NT / 64 * 3];
+    int turn = 0;
     const int lane = threadIdx.x % G, grp = threadIdx.x / G;
     const int nfull = C / E, rem = C % E;
     const float inv_c = 1.f / (float)C;
@@ -203,7 +205,8 @@ __global__ __launch_bounds__(NT) void layer_norm_bwd_kernel(const T* dy, long ld
         s[0] += xht;
         s[1] += gt;
         s[2] += gt * xht;
-        row_sums<NT, G, 3>(s, red);
+        row_sums<NT, G, 3>(s, red[turn]);
+        turn ^= 1;
         keep_packed<T, NV>(qx.q);
         keep_packed<T, NV>(qd.q);
         const float off = s[0] * inv_c, mg = s[1] * inv_c, mgx = s[2] * inv_c - mg * off;
