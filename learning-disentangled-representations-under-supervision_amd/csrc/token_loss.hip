@@ -5,6 +5,8 @@
 // against them. HBM-bound: two to five flops and one v_exp_f32 per element. One workgroup holds a row in registers, so
 // a loss whose row gradient needs nothing but the row (the policy loss) reads the logits once and writes the gradient
 // once. Rows of weight zero (the padding of a batch) are not read: their log-probability and gradient are zeros.
+// Loss and gradient of 10496 x 50000 bf16 rows: 414 us with all of them live (5.1 TB/s, what a copy reaches), 313 us with
+// half of them padding; log-probabilities alone 5.3 to 5.7 TB/s; the gradient pass from saved statistics 5.4 to 6.0 TB/s.
 #include "rows.h"
 
 namespace {
@@ -91,8 +93,8 @@ struct RowScalars {
         const double kept = A > 0.f ? (ratio > hi ? hi : ratio) : (ratio < lo ? lo : ratio);
         double loss = -kept * (double)A;
         if (a.ref_logp) {
-            const double k = (double)ref_logp - lp;
-            loss += (double)a.kl_coef * (expm1(k) - k);
+            const double k = (double)ref_logp - lp, e = expm1(k);
+            loss += (double)a.kl_coef * (e == INFINITY ? e : e - k);
         }
         a.row_loss[row] = loss * (double)w;
     }
@@ -161,6 +163,8 @@ __device__ __forceinline__ void load_all(Piece<T> (&q)[NV], const T* x, const Cu
 }
 
 // One workgroup per row, the row in registers: NV 16-byte pieces per thread and one single element of its ragged ends.
+// Rows of more than 1024 pieces take 1024 threads, two rows per CU: 10496 x 50000 bf16 413 us all live, 314 us half padding;
+// with 512 threads and three rows per CU 398 and 328 us (a padded batch is the ordinary one), 256 and 640 in between.
 template <typename T, int NT, int NV>
 __global__ __launch_bounds__(NT) void row_kernel(const RowArgs a) {
     constexpr int E = Piece<T>::E, NW = NT / 64;
@@ -495,9 +499,6 @@ template <typename T>
 int launch_rows(hipStream_t s, RowArgs a, int64_t M, bool* done) {
     const int n = cgn_cdiv(a.V, Piece<T>::E);
     *done = true;
-#ifdef VAR
-    VAR
-#endif
     if (n <= 256 * 1) return launch_row<T, 256, 1>(s, a, M);
     if (n <= 256 * 2) return launch_row<T, 256, 2>(s, a, M);
     if (n <= 256 * 4) return launch_row<T, 256, 4>(s, a, M);

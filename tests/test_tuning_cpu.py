@@ -251,6 +251,9 @@ def test_entry_points_refuse_bad_arguments():
     assert lib.cgn_clip_grads(None, tb, n, 0, 1.0, 1.0, None, P, nb.value) == BAD
     tb, n = table((4096, 0, 1, 4, 0, 0, 0))
     assert lib.cgn_clip_grads(None, tb, n, 0, 1.0, 1.0, P, P, 1 << 20) == BAD  # no destination
+    for one in (1, 4096, 4097, 1 << 20, (1 << 22) + 1, (1 << 25) + 1, 64000000):  # one tensor: at most 1024 partials
+        tb, n = table((4096, 4096, 1, one, 0, 0, 0))
+        assert lib.cgn_grad_norm_workspace(tb, n, 0, C.byref(nb)) == _lib.CGN_OK and nb.value <= 8 * 1024 + 8
     for second, ok in ((4096 + 16, True), (4096 + 12, False), (4096, False)):  # two tensors of 4, apart or not
         tb, n = table((4096, 4096, 1, 4, 0, 0, 0), (second, second, 1, 4, 0, 0, 0))
         assert lib.cgn_grad_norm_workspace(tb, n, 1, C.byref(nb)) == (_lib.CGN_OK if ok else BAD)

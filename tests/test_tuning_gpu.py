@@ -73,7 +73,7 @@ def norm_ref(x, w, b, eps, dy=None):
 NORM_SIZES = [(1, 1), (3, 1), (1, 2), (5, 7), (2, 8), (33, 9), (64, 33), (7, 63), (9, 64), (4, 65), (130, 127), (3, 256),
               (5, 257), (3, 300), (65, 512), (6, 513), (4, 600), (10, 800), (37, 825), (300, 1024), (5, 1025), (2, 2047),
               (3, 2049), (2, 4096), (3, 4097), (2, 8191), (2, 8192), (2100, 40), (7, 1500), (9, 3000),
-              (11, 8000), (40, 500), (700, 20)]
+              (11, 8000), (40, 500), (700, 20), (20, 1500), (13, 825), (16, 825), (17, 825)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -415,6 +415,17 @@ def test_banned_tokens(dev, V, dtype):
     assert logp[1].isnan()
 
 
+def test_kl_of_a_banned_target_is_infinite(dev):
+    """e^k - k - 1 grows without bound as the token's probability goes to zero: infinity, and no NaN from inf - inf."""
+    x, t, A, w, old, ref = make_policy(6, 300, F32, 11, dev, dead=0.0)
+    x[2, t[2]] = -float("inf")
+    for weight in (w, w * (torch.arange(6, device=dev) != 2)):
+        loss, logp = ops.policy_loss(x, t, A, weight, ref_logp=ref, kl_coef=0.1)
+        assert torch.isfinite(loss) if float(weight[2]) == 0 else float(loss) == float("inf")
+    loss, logp = ops.policy_loss(x, t, A, w, ref_logp=ref, kl_coef=0.0)  # -lp A alone is no part of the loss: rho = 1
+    assert torch.isfinite(loss) and float(logp[2]) == -float("inf")
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("V", [37, 5001, 140003])
 @pytest.mark.parametrize("base", [-3.0e38, -1.0e30, -2.0e6, 1.0e5, 2.0e6, 1.0e30, 3.0e38])
@@ -641,6 +652,7 @@ def test_clip_layouts(dev):
     b16 = torch.randn(40000, device=dev, generator=g).to(BF16)
     views = [buf[1:1 + 20 * 828].view(20, 828)[:, :825], buf[17000:17000 + 12].view(3, 4).t(),
              buf[18001:18001 + 30 * 31].view(30, 31)[:, 1:30], buf[20001:20008],
+             buf[21000:21000 + 9000 * 2].view(9000, 2)[:, :1], buf[39100:39100 + 100 * 9].view(100, 9)[:, 2:5],
              b16[3:3 + 50 * 130].view(50, 130)[:, :129], b16[7001:7001 + 60].view(5, 4, 3).permute(2, 0, 1)]
     keep, bkeep, gk = buf.clone(), b16.clone(), [v.clone() for v in views]
     want = norm64(views)
