@@ -479,7 +479,7 @@ def pair_ref(x, t, w, ref, beta, smooth, it):
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("P,T,V", [(1, 1, 5), (1, 3, 1000), (3, 1, 33), (2, 65, 77), (5, 21, 300), (2, 7, 20001),
-                                   (1, 2, 131075), (70, 3, 40), (70, 65, 9)])
+                                   (1, 2, 131075), (70, 3, 40), (70, 65, 9), (9, 2, 300), (600, 1, 12), (2100, 1, 5)])
 def test_preference_loss(dev, P, T, V, dtype):
     x, t, g = make_rows(2 * P * T, V, dtype, P * 1009 + T * 101 + V, dev)
     n = torch.randint(0, T + 1, (2 * P, 1), device=dev, generator=g)
