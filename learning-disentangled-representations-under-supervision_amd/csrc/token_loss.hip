@@ -66,10 +66,14 @@ struct RowScalars {
         xt = t >= 0 && t < a.V ? Piece<T>::one((const T*)a.logits + row * a.ld + t) : NAN;
     }
 
+    // The ratio to the policy that sampled the token. Without one it is 1, but for a token without a log-probability (a
+    // target outside the vocabulary, a NaN logit): its loss and its gradient are NaN. (-inf has one: a ratio of 1.)
+    static __device__ __forceinline__ double ratio_1(double lp) { return lp == lp ? 1.0 : lp; }
+
     // d loss / d lp. expm1: k is small where the two policies agree.
     __device__ __forceinline__ float slope(const RowArgs& a, float w, float inv_tau, float m, float z) const {
         const double lp = ((double)xt - (double)m) * (double)inv_tau - (double)logf(z);
-        const float ratio = a.old_logp ? expf((float)(lp - (double)old_logp)) : 1.f;
+        const float ratio = a.old_logp ? expf((float)(lp - (double)old_logp)) : (float)ratio_1(lp);
         const bool cut = (A > 0.f && ratio > 1.f + a.clip_hi) || (A < 0.f && ratio < 1.f - a.clip_lo);
         float g = cut ? 0.f : -ratio * A;
         if (a.ref_logp) g -= a.kl_coef * expm1f((float)((double)ref_logp - lp));
@@ -87,7 +91,7 @@ struct RowScalars {
         }
         if (!a.advantage) return;
         if (a.coef) a.coef[row] = g;
-        const double ratio = a.old_logp ? exp(lp - (double)old_logp) : 1.0;
+        const double ratio = a.old_logp ? exp(lp - (double)old_logp) : ratio_1(lp);
         const double lo = 1.0 - (double)a.clip_lo, hi = 1.0 + (double)a.clip_hi;
         // the smaller of ratio A and clip(ratio) A
         const double kept = A > 0.f ? (ratio > hi ? hi : ratio) : (ratio < lo ? lo : ratio);

@@ -386,6 +386,39 @@ def test_masked_rows_strides_and_bad_values(dev, V, extra, shift, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [300, 20001, 140003])
+@pytest.mark.parametrize("sampled_here", [True, False])
+def test_policy_rows_without_a_log_probability(dev, V, sampled_here, dtype):
+    """A target outside the vocabulary and a NaN logit in rows that count: NaN in the loss, in the row's log-probability and
+    in every column of its gradient, on-policy (no old log-probabilities) too, fused and through autograd, on both sides
+    of what a workgroup's registers hold. A token of probability zero is none of these: its ratio stays 1."""
+    M = 8
+    x, t, A, w, old, _ = make_policy(M, V, dtype, V, dev, dead=0.0)
+    t[1], t[4] = V, -100                                       # an index behind the end, the usual ignored index
+    x[6, (int(t[6]) + 1) % V] = float("nan")
+    x[3, int(t[3])] = -float("inf")
+    A[4] = 0.0
+    bad = torch.zeros(M, dtype=torch.bool, device=dev)
+    bad[[1, 4, 6]] = True
+    kw = dict(old_logp=None if sampled_here else old)
+    for only in (None, 1, 4, 6):                               # all rows, and each of the bad ones alone
+        wi = w if only is None else torch.where(torch.arange(M, device=dev) == only, w, 0.0)
+        hit = bad & (wi != 0)
+        d = torch.empty_like(x)
+        loss, logp = ops.policy_loss(x, t, A, wi, dlogits=d, **kw)
+        xr = x.clone().requires_grad_()
+        loss2, logp2 = hnn.policy_loss(xr, t, A, wi, **kw)
+        loss2.backward()
+        assert loss.isnan().all() and loss2.isnan(), only
+        for lp, grad in ((logp, d), (logp2, xr.grad)):
+            assert torch.equal(lp.isnan(), hit), only
+            assert grad[hit].isnan().all() and torch.isfinite(grad[~hit].float()).all(), only
+    wi = torch.where(bad, 0.0, w)                              # without them
+    loss, logp = ops.policy_loss(x, t, A, wi, **kw)
+    assert torch.isfinite(loss).all() and float(logp[3]) == -float("inf")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("V", [40, 3000, 140000])
 def test_banned_tokens(dev, V, dtype):
     """-inf and the type's lowest value in rows that count: those tokens have probability and gradient zero."""
