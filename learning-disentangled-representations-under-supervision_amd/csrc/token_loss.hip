@@ -445,10 +445,12 @@ __global__ __launch_bounds__(PAIR_NT) void pair_kernel(const double* __restrict_
     const double neg = mg >= 0.0 ? ex / (1.0 + ex) : 1.0 / (1.0 + ex);
     const double up = -(beta / (double)P) * ((1.0 - smooth) * neg - smooth * pos);
     if ((threadIdx.x & 127) == 0) {
-        // (fmin drops a NaN margin; the loss keeps it)
-        const double one = -((1.0 - smooth) * (fmin(mg, 0.0) - l1) + smooth * (fmin(-mg, 0.0) - l1));
+        double ls = (1.0 - smooth) * (fmin(mg, 0.0) - l1);
+        // left out without smoothing: log sig(-m) is -inf where the model cannot produce the rejected sentence, and such a
+        // pair has a loss of 0
+        if (smooth > 0.0) ls += smooth * (fmin(-mg, 0.0) - l1);
         margin[p] = (float)mg;
-        pair_loss[p] = sum[slot] = mg != mg ? mg : one;
+        pair_loss[p] = sum[slot] = mg != mg ? mg : -ls;  // (fmin drops a NaN margin; the loss keeps it)
     }
     if (coef)
         for (int t = lane; t < T; t += 64) coef[seq * T + t] = (float)((side ? -up : up) * (double)weight[seq * T + t]);

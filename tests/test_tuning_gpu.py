@@ -552,6 +552,50 @@ def test_preference_loss_far_margins(dev):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("P,T,V", [(1, 1, 40), (3, 4, 3000), (12, 2, 300), (3, 1, 140003)])
+def test_preference_loss_of_impossible_sentences(dev, P, T, V, dtype):
+    """A sentence with a banned word (logit -inf) has log-probability -inf. Rejected, its pair is decided: margin +inf, loss
+    -log sigmoid(inf) = 0 and no gradient without smoothing, +inf with it. Chosen: margin -inf, loss +inf. The gradients
+    are finite: sigmoid(+-inf) is 0 or 1. The other pairs' numbers are as without it."""
+    x, t, g = make_rows(2 * P * T, V, dtype, 17 * P + V, dev)
+    w = 1 + torch.rand(2 * P, T, device=dev, generator=g)
+    S = (softmax_ref(x, t, 1.0)[0].view(2 * P, T) * w).sum(1)
+    ref = (S + 3 * torch.randn(2 * P, device=dev, generator=g)).float()
+    odd, beta, inf = P - 1, 0.3, float("inf")
+    rest = [p for p in range(P) if p != odd]
+    sents = rest + [P + p for p in rest]
+    for side, smooth in ((1, 0.0), (1, 0.1), (0, 0.0), (0, 0.1)):
+        xb = x.clone()
+        row = (side * P + odd) * T + T // 2
+        xb[row, int(t[row])] = -inf
+        d = torch.full_like(x, float("nan"))
+        loss, margin, seq = ops.preference_loss(xb, t, w, ref, beta=beta, label_smoothing=smooth, dlogits=d)
+        alone = ops.preference_loss(xb, t, w, ref, beta=beta, label_smoothing=smooth)
+        assert all(torch.equal(a, b) for a, b in zip(alone, (loss, margin, seq)))
+        assert float(margin[odd]) == (inf if side else -inf) and float(seq[side * P + odd]) == -inf
+        total, band = 0.0, 0.0
+        if rest:
+            pick = torch.tensor([s * T + i for s in sents for i in range(T)], device=dev)
+            want = pair_ref(x[pick], t[pick], w[sents], ref[sents], beta, smooth, 1.0)
+            f = len(rest) / P
+            total, band = float(want["loss"]) * f, want["dl"] * f
+            check_dlogits(d[pick], want["d"] * f, want["tol"] * f, "the other pairs' dlogits")
+        if side and not smooth:
+            assert abs(float(loss) - total) <= band + 2 * U * abs(total), (side, smooth)
+        else:
+            assert float(loss) == inf, (side, smooth)
+        # d loss / dS of the chosen sentence, minus that of the rejected one
+        up = beta / P * smooth if side else -beta / P * (1 - smooth)
+        own = torch.tensor([s * T + i for s in (odd, P + odd) for i in range(T)], device=dev)
+        _, ls, _ = softmax_ref(xb[own], t[own], 1.0)
+        coef = (w[[odd, P + odd]].double() * torch.tensor([[up], [-up]], device=dev)).view(-1)
+        want, tol = dlogits_ref(ls, t[own], coef, 1.0, torch.zeros_like(coef), coef.abs())
+        check_dlogits(d[own], want, tol, "dlogits of the pair")
+        if up == 0:
+            assert not d[own].any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_loss_modules(dev, dtype):
     """The differentiable forms: the gradient times the upstream one, and (fp32) against differences."""
     M, V = 12, 301
