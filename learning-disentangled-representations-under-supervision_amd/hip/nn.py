@@ -403,7 +403,7 @@ class _PolicyLossFn(torch.autograd.Function):
         ctx.save_for_backward(logits, target, weight, stats, coef)
         ctx.inv_tau = inv_tau
         ctx.mark_non_differentiable(logp)
-        return loss.view(()), logp
+        return loss.squeeze_(), logp  # (no view: a training loop divides and adds to its loss in place)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -430,7 +430,7 @@ class _PreferenceLossFn(torch.autograd.Function):
         ctx.save_for_backward(logits, target, weight, stats, coef)
         ctx.inv_tau = inv_tau
         ctx.mark_non_differentiable(margin, seq_logp)
-        return loss.view(()), margin, seq_logp
+        return loss.squeeze_(), margin, seq_logp
 
     @staticmethod
     @torch.autograd.function.once_differentiable

@@ -631,6 +631,41 @@ def test_loss_modules(dev, dtype):
         assert abs(slope(f) - float((grad.double() * v.double()).sum())) <= 30 * float(w.sum()) * (h * h + 64 * U / h)
 
 
+@pytest.mark.parametrize("form", ["policy", "preference"])
+def test_losses_take_in_place_arithmetic(dev, form):
+    """What a training loop does with a loss, loss /= steps and loss += another one, and with the numbers beside it: they
+    are tensors of their own, from the differentiable forms and from the explicit ones."""
+    M, V = 12, 40
+    x, t, A, w, old, _ = make_policy(M, V, F32, 5, dev, dead=0.0)
+    sref = torch.zeros(4, device=dev)
+
+    def call(m, v):
+        return m.policy_loss(v, t, A, w, old_logp=old) if form == "policy" else m.preference_loss(v, t, w.view(4, 3), sref,
+                                                                                                   beta=0.2)
+
+    plain = x.clone().requires_grad_()
+    loss = call(hnn, plain)[0] / 4
+    (loss + plain.square().mean()).backward()
+    xr = x.clone().requires_grad_()
+    got = call(hnn, xr)
+    beside = [b.clone() for b in got[1:]]
+    total = got[0]
+    total /= 4
+    total += xr.square().mean()
+    for b in got[1:]:
+        b.mul_(2.0)
+    total.backward()
+    assert torch.equal(total.detach(), (loss + plain.square().mean()).detach())
+    close(xr.grad, plain.grad, 2 * U * plain.grad.double().abs(), "gradient")  # (the two parts may be added in either order)
+    assert all(torch.equal(b, 2 * k) for b, k in zip(got[1:], beside))
+    explicit = call(ops, x)
+    aux = torch.ones((), device=dev, requires_grad=True)
+    total = explicit[0]
+    total += aux
+    total.sum().backward()
+    assert float(aux.grad) == 1.0 and not any(b.requires_grad for b in explicit[1:])
+
+
 def test_long_offsets(dev):
     """More than 2^31 elements of logits: the last rows are read and written where they are."""
     V, M = 50000, 43100
