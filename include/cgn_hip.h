@@ -616,7 +616,8 @@ int cgn_cast_bf16_f32(void* stream, const float* src, cgn_axis rows, int32_t n_r
 int cgn_layer_norm_fwd(void* stream, const void* x, int64_t ldx, int64_t R, int32_t C, int32_t bf16, const float* weight,
                        const float* bias, float eps, void* y, int64_t ldy, float* mean, float* rstd);
 /* Its backward pass, from the statistics of the forward pass: dx (nullable; may be dy's or x's own buffer) and
- * dweight / dbias = beta * itself + the sums over the rows (nullable; R == 0 gives sums of zero).
+ * dweight / dbias = beta * itself + the sums over the rows (nullable; R == 0 gives sums of zero). The two overlap neither
+ * each other (CGN_ERR_INVALID_ARG) nor anything else of the call.
  * workspace (with dweight or dbias): what cgn_layer_norm_bwd_workspace says for the shape (host call; may be nothing). */
 int cgn_layer_norm_bwd_workspace(int64_t R, int32_t C, int32_t bf16, int64_t* bytes);
 int cgn_layer_norm_bwd(void* stream, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t R, int32_t C,

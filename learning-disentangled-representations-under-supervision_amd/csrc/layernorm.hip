@@ -350,6 +350,8 @@ int launch_bwd(hipStream_t s, const void* dy, int64_t lddy, const void* x, int64
         return CGN_OK;
     }
     if (params && !alone && nb * 2 * C * 4 > part_bytes) return CGN_ERR_WORKSPACE;
+    // the two are written by threads that do not know of each other
+    if (dw && db && (uintptr_t)dw < (uintptr_t)(db + C) && (uintptr_t)db < (uintptr_t)(dw + C)) return CGN_ERR_INVALID_ARG;
     if (nb > 0) {
         hipLaunchKernelGGL((layer_norm_bwd_kernel<T, NT, G, NV>), dim3((unsigned)nb), dim3(NT), 0, s, (const T*)dy,
                            (long)lddy, (const T*)x, (long)ldx, (long)R, C, w, mean, rstd, (T*)dx, (long)lddx,

@@ -1471,6 +1471,12 @@ def _own_or_apart(dst, ldd, src, lds, rows, cols, name):
              "%s must be the source's own buffer or lie apart from it" % name)
 
 
+def _overlap(t, n, u, m):
+    """Whether the first n elements from t's start on share memory with the first m from u's."""
+    a, b = t.data_ptr(), u.data_ptr()
+    return n > 0 and m > 0 and a < b + m * u.element_size() and b < a + n * t.element_size()
+
+
 def _vector(t, n, name, dev):
     _chk_f32(t, name)
     if t.numel() != n or not t.is_contiguous() or t.device != dev:
@@ -1513,7 +1519,7 @@ def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5, out=None):
 def layer_norm_bwd(dy, x, weight, mean, rstd, dx=None, dweight=None, dbias=None, beta=0.0, params=True):
     """Backward of layer_norm_fwd: (dx, dweight, dbias). dx: its destination (dy's or x's own buffer is allowed), None for
     a new tensor, False to leave it out. params: form dweight / dbias (= beta * what they hold + the sums over the rows
-    where destinations are given; dweight is None for weight None)."""
+    where destinations are given, which overlap nothing else of the call; dweight is None for weight None)."""
     b16, R, Cn, ldx = _layer_norm_rows(x, "x")
     dev = x.device
     _req(dy.shape == x.shape and dy.dtype == x.dtype and dy.device == dev, "dy must be like x")
@@ -1539,6 +1545,7 @@ def layer_norm_bwd(dy, x, weight, mean, rstd, dx=None, dweight=None, dbias=None,
         if dweight is None and dbias is None and weight is not None:
             dweight, dbias = alloc((2, Cn), dev).unbind(0)
         else:
+            given = [t for t in (dweight, dbias) if t is not None]
             if dweight is not None:
                 _vector(dweight, Cn, "dweight", dev)
             elif weight is not None:
@@ -1547,6 +1554,12 @@ def layer_norm_bwd(dy, x, weight, mean, rstd, dx=None, dweight=None, dbias=None,
                 _vector(dbias, Cn, "dbias", dev)
             else:
                 dbias = alloc((Cn,), dev)
+            spans = [(x, ldx, Cn, R), (dy, lddy, Cn, R), (dx, lddx, Cn, R), (weight, Cn, Cn, 1), (mean, R, R, 1),
+                     (rstd, R, R, 1)]
+            spans = [(t, (rows - 1) * ld + n if rows else 0) for t, ld, n, rows in spans if t is not None]
+            _req(not any([_overlap(d, Cn, t, n) for d in given for t, n in spans])
+                 and not (len(given) == 2 and _overlap(dweight, Cn, dbias, Cn)),
+                 "dweight and dbias must not overlap each other, an operand or dx")
         nb = C.c_int64()
         _lib.check(_lib.load().cgn_layer_norm_bwd_workspace(R, Cn, b16, C.byref(nb)), "cgn_layer_norm_bwd_workspace")
         if nb.value:

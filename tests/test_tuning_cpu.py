@@ -93,6 +93,51 @@ def test_layer_norm_refusals(host):
     assert len(host) == 4
 
 
+def test_layer_norm_parameter_destinations_lie_apart(host):
+    """dweight and dbias are written by threads of their own while the operands are read: given destinations overlap
+    neither each other nor an operand nor dx."""
+    x, dy, v, w = torch.zeros(4, 8), torch.zeros(4, 8), torch.zeros(8), torch.ones(8)
+    mean, rstd, buf, wide = torch.zeros(4), torch.zeros(4), torch.zeros(64), torch.zeros(4, 16)
+    stats = torch.zeros(16)
+    call = lambda dweight, dbias, **k: ops.layer_norm_bwd(k.pop("dy", dy), k.pop("x", x), k.pop("w", w),  # noqa: E731
+                                                          k.pop("mean", mean), k.pop("rstd", rstd), dweight=dweight,
+                                                          dbias=dbias, **k)
+    bad = [
+        lambda: call(v, v),                                            # one tensor for both
+        lambda: call(buf[:8], buf[7:15]),
+        lambda: call(w, v),
+        lambda: call(None, w),
+        lambda: call(buf[4:12], None, w=buf[:8]),
+        lambda: call(x.view(-1)[:8], v),
+        lambda: call(v, dy.view(-1)[24:]),
+        lambda: call(v, buf[31:39], dy=buf[:32].view(4, 8)),
+        lambda: call(wide.view(-1)[48:56], None, x=wide[:, :8]),
+        lambda: call(v, stats[2:10], mean=stats[:4]),
+        lambda: call(stats[6:14], v, rstd=stats[4:8]),
+        lambda: call(buf[:8], v, dx=buf[:32].view(4, 8)),
+    ]
+    for k, f in enumerate(bad):
+        with pytest.raises(ValueError, match="overlap"):
+            f()
+            raise AssertionError("case %d was taken" % k)
+    assert not host
+    call(buf[:8], buf[8:16])
+    call(buf[32:40], buf[40:48], x=buf[:32].view(4, 8), dx=dy)
+    call(None, v)
+    call(v, None, dx=x)
+    assert len(host) == 4
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the pointers are dummies: only where nothing can be launched")
+def test_layer_norm_entry_point_refuses_one_destination_for_both():
+    lib, nb = _lib.load(), C.c_int64()
+    for R in (3, 2000):  # one workgroup, many
+        assert lib.cgn_layer_norm_bwd_workspace(R, 8, 0, C.byref(nb)) == _lib.CGN_OK
+        for off in (-28, -4, 0, 4, 28):
+            assert lib.cgn_layer_norm_bwd(None, P, 8, P, 8, R, 8, 0, None, P, P, None, 8, C.c_void_p(8192),
+                                          C.c_void_p(8192 + off), 0.0, P, nb.value) == BAD, (R, off)
+
+
 def test_token_loss_refusals(host):
     x, i = torch.zeros(4, 8), torch.zeros(4, dtype=torch.int64)
     v, w = torch.zeros(4), torch.ones(2, 2)
