@@ -422,13 +422,13 @@ __global__ __launch_bounds__(NT) void row_grad_kernel(const GradArgs a) {
 // launch less: 2 us of 26 for a single pair); more pairs take a workgroup each (64 pairs of 41 tokens in one: 20 us longer).
 constexpr int PAIR_W = 8, PAIR_NT = 128 * PAIR_W;
 __global__ __launch_bounds__(PAIR_NT) void pair_kernel(const double* __restrict__ lp64, const float* __restrict__ weight,
-                                                       const float* __restrict__ ref, int P, int T, double beta,
+                                                       const float* __restrict__ ref, int p0, int P, int T, double beta,
                                                        double smooth, float* __restrict__ seq_logp,
                                                        float* __restrict__ margin, double* __restrict__ pair_loss,
                                                        float* __restrict__ coef, float* __restrict__ loss) {
     __shared__ double S[PAIR_W][2], sum[PAIR_W];
     const int slot = threadIdx.x >> 7, side = threadIdx.x >> 6 & 1, lane = threadIdx.x & 63;
-    const int p = blockIdx.x * (blockDim.x >> 7) + slot;  // (the grid covers the pairs exactly)
+    const int p = p0 + blockIdx.x * (blockDim.x >> 7) + slot;  // (the grids cover the pairs exactly)
     const long seq = (long)side * P + p;
     double s = 0.0;
     for (int t = lane; t < T; t += 64) s += lp64[seq * T + t];
@@ -454,7 +454,7 @@ __global__ __launch_bounds__(PAIR_NT) void pair_kernel(const double* __restrict_
     }
     if (coef)
         for (int t = lane; t < T; t += 64) coef[seq * T + t] = (float)((side ? -up : up) * (double)weight[seq * T + t]);
-    if (gridDim.x > 1) return;
+    if (!loss) return;  // summed elsewhere: this is not the only workgroup
     __syncthreads();
     if (threadIdx.x == 0) {
         double t = 0.0;
@@ -668,9 +668,13 @@ extern "C" int cgn_preference_loss(void* stream, const cgn_token_rows* r, int32_
     int rc = run_rows(s, a, r->M, r->bf16 != 0, &done);
     if (rc != CGN_OK) return rc;
     const bool few = P <= PAIR_W;
-    hipLaunchKernelGGL(pair_kernel, dim3(few ? 1 : P), dim3(few ? 128 * P : 128), 0, s, lp64, r->weight, ref_logp, P, T, beta,
-                       label_smoothing, seq_logp, margin, pair_loss, coef, loss);
-    CGN_LAUNCH_CHECK();
+    for (int64_t p0 = 0; p0 < P; p0 += GRID_THREADS / 128) {
+        const int64_t n = P - p0 < GRID_THREADS / 128 ? P - p0 : GRID_THREADS / 128;
+        hipLaunchKernelGGL(pair_kernel, dim3(few ? 1 : (unsigned)n), dim3(few ? 128 * P : 128), 0, s, lp64, r->weight,
+                           ref_logp, (int)p0, P, T, beta, label_smoothing, seq_logp, margin, pair_loss, coef,
+                           few ? loss : nullptr);
+        CGN_LAUNCH_CHECK();
+    }
     if (dlogits) return row_gradient(s, r, stats, coef, nullptr, dlogits, ldd, few ? nullptr : pair_loss, P, loss);
     // (with as many threads as sum it in the gradient's launch: the same order, the same bits)
     return few ? CGN_OK : run_sum<GRAD_NT>(s, pair_loss, P, 1.0 / P, loss);

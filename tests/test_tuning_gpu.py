@@ -706,6 +706,29 @@ def test_more_rows_than_a_grid_holds(dev):
     check_dlogits(d, want["d"], want["d_tol"], "dlogits")
 
 
+def test_more_pairs_than_a_grid_holds(dev):
+    """2^25 pairs and some of one token each, at 128 threads a pair: more than one launch of the pair kernel."""
+    P, V, beta = (1 << 25) + 3, 2, 0.5
+    x = torch.randn(2 * P, V, device=dev, generator=gen(1))
+    t = torch.randint(0, V, (2 * P,), device=dev, generator=gen(2))
+    w = torch.rand(2 * P, 1, device=dev, generator=gen(3)) + 0.5
+    ref = torch.randn(2 * P, device=dev, generator=gen(4))
+    d = torch.full_like(x, float("nan"))
+    loss, margin, seq = ops.preference_loss(x, t, w, ref, beta=beta, dlogits=d)
+    lp, ls, band = softmax_ref(x, t, 1.0)
+    S, dS = lp * w[:, 0].double(), band * w[:, 0].double()
+    close(seq, S, dS + U * S.abs(), "seq_logp")
+    gain = S - ref.double()
+    m, dm = beta * (gain[:P] - gain[P:]), beta * (dS[:P] + dS[P:])
+    close(margin, m, dm + U * m.abs(), "margin")
+    want = float(-torch.nn.functional.logsigmoid(m).mean())
+    assert abs(float(loss) - want) <= float(dm.mean()) + 2 * U * want
+    up, dup = -(beta / P) * torch.sigmoid(-m), beta / P * dm / 4
+    coef, cerr = torch.cat((up, -up)) * w[:, 0].double(), torch.cat((dup, dup)) * w[:, 0].double()
+    wd, tol = dlogits_ref(ls, t, coef, 1.0, torch.zeros_like(band), coef.abs())
+    check_dlogits(d, wd, tol + 2 * cerr[:, None], "dlogits")  # (p + 1 at the target is at most 2)
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # gradient norm and clipping
 # ---------------------------------------------------------------------------------------------------------------------
