@@ -140,6 +140,39 @@ def test_layer_norm_strides_in_place_and_optional_parts(dev, C, extra, shift, dt
     close(dx, ref["dx"], ref["dx_tol"] + half(dx) * (ref["dx"].abs() + ref["dx_tol"]), "dx without parameters")
 
 
+# more rows than a launch has groups for (every group walks several, the forward pass past 8192 workgroups, the backward
+# pass past what is resident), remainders of the grids, and matrices on both sides of the 128 MB that are streamed from on
+LARGE_NORMS = [(300000, 24), (40000, 600), (9001, 1100), (9000, 2100), (8200, 4100), (45001, 825), (83001, 825)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("R,C", LARGE_NORMS)
+def test_layer_norm_of_many_rows(dev, R, C, dtype):
+    g = gen(R + C)
+    x = (torch.randn(R, C, device=dev, generator=g) * 2 + torch.randn(R, 1, device=dev, generator=g)).to(dtype)
+    dy = torch.randn(R, C, device=dev, generator=g).to(dtype)
+    w, b = torch.randn(C, device=dev, generator=g), torch.randn(C, device=dev, generator=g)
+    y, mean, rstd = ops.layer_norm_fwd(x, w, b, 1e-5)
+    dx, dw, db = ops.layer_norm_bwd(dy, x, w, mean, rstd)
+    ref = norm_ref(x, w, b, 1e-5, dy)
+    close(mean, ref["mu"], 42 * U * x.double().abs().mean(-1), "mean")
+    close(rstd, ref["r"], 64 * U * ref["r"], "rstd")
+    ytol = 64 * U * (ref["xh"].abs() * w.abs() + w.abs() + b.abs())
+    close(y, ref["y"], ytol + half(y) * (ref["y"].abs() + ytol), "y")
+    close(dx, ref["dx"], ref["dx_tol"] + half(dx) * (ref["dx"].abs() + ref["dx_tol"]), "dx")
+    # a column's additions in fp32: at most 41 rows in a group of a workgroup's 4, or 10 in one of its 64, and then the
+    # groups: below 96 (64 bits from there on); 64 u an element for xh itself
+    close(dw, ref["dw"], ref["dw_tol"] * 160 / 128, "dweight")
+    close(db, ref["db"], ref["db_tol"], "dbias")
+    del ref, ytol
+    for over in (0, 1):  # in place: the next rows' loads are in flight while a row is written
+        di, xi = dy.clone(), x.clone()
+        got = ops.layer_norm_bwd(di, xi, w, mean, rstd, dx=(di, xi)[over])
+        assert torch.equal(got[0], dx) and torch.equal(got[1], dw) and torch.equal(got[2], db)
+    xi = x.clone()
+    assert torch.equal(ops.layer_norm_fwd(xi, w, b, 1e-5, out=xi)[0], y)
+
+
 def test_layer_norm_keeps_precision_far_from_zero(dev):
     """A row's mean 1000 times its spread: the statistics' second sum takes out what the first one's rounding left."""
     g = gen(5)
@@ -326,6 +359,14 @@ def test_policy_loss(dev, M, V, dtype):
         ops.policy_loss(xi, t, A, w, old_logp=o, ref_logp=ref, clip=(0.2, 0.3), kl_coef=kl, inv_tau=it, dlogits=xi)
         assert torch.equal(xi, d)
         check_dlogits(ops.token_logp_bwd(x, t, stats, coef, weight=w, inv_tau=it), want["d"], want["d_tol"], "saved")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [12289, 14001, 16384])
+def test_rows_of_four_pieces_a_thread(dev, V, dtype):
+    """Vocabularies of 12289 to 16384 words in fp32 have a register variant of their own."""
+    test_token_logp(dev, 2, V, dtype)
+    test_policy_loss(dev, 3, V, dtype)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -780,6 +821,26 @@ def test_clip_many_tensors(dev, count):
     assert torch.equal(ops.grad_norm(keep, grad_scale=-0.25), norm)
 
 
+@pytest.mark.parametrize("kind", [2.0, float("inf")])
+@pytest.mark.parametrize("sizes", [[(5000001,), (1234567,), (3,), (1999, 1501), (0,), (70001,)],
+                                   [(17000003,), (8193,), (16900001,), (4000, 1023), (2,), (300, 12)]])
+def test_clip_large_lists(dev, sizes, kind):
+    """More elements than the smallest share of a workgroup leaves to 1024 of them (every thread makes several trips), and
+    more than 32 M (written past the caches); sizes off the shares, mixed types, one matrix with a row stride."""
+    grads = grads_of(sizes, dev, len(sizes))
+    wide = torch.randn(sizes[3][0], sizes[3][1] + 5, device=dev, generator=gen(3))
+    grads[3] = wide[:, :sizes[3][1]]
+    keep, gap = [t.clone() for t in grads], wide[:, sizes[3][1]:].clone()
+    want = norm64(grads, kind)
+    out = [torch.full_like(t, 9.0) for t in keep]
+    out[3] = torch.full_like(wide, 9.0)[:, :sizes[3][1]]
+    norm = ops.clip_grad_norm(grads, want / 8, kind, out=out)
+    check_clipped(out, keep, norm, want, want / 8)
+    assert all(torch.equal(a, b) for a, b in zip(grads, keep))
+    assert torch.equal(ops.clip_grad_norm(grads, want / 8, kind), norm)
+    assert all(torch.equal(a, b) for a, b in zip(grads, out)) and torch.equal(wide[:, sizes[3][1]:], gap)
+
+
 def test_clip_layouts(dev):
     """Padded matrix views, permuted pieces, odd starts; what lies between the rows stays as it is."""
     g = gen(2)
@@ -866,6 +927,39 @@ def test_adam_clipped(dev, n):
     assert ops.adam(p, grad, m, v, 1e-2, 7) is None
 
 
+def test_adam_of_streamed_arenas(dev):
+    """Arenas of 32 M elements and more pass the caches by: the update against its formula in 64 bits, and bit for bit
+    against the same arena updated in slices below that size."""
+    n, step, gs = (32 << 20) + 4103, 7, 0.5
+    g = gen(1)
+    p, grad, m, v = [torch.randn(n, device=dev, generator=g) for _ in range(4)]
+    m, v = m * 0.1, v.square()
+    f = lambda x: float(torch.tensor(x, dtype=F32))  # noqa: E731
+    lr, b1, b2, eps = f(1e-2), f(0.9), f(0.999), f(1e-8)
+    a, b = [[t.clone() for t in (p, m, v)] for _ in range(2)]
+    assert ops.adam(a[0], grad, a[1], a[2], 1e-2, step, grad_scale=gs) is None
+    for lo, hi in ((0, 12 << 20), (12 << 20, (25 << 20) + 4), ((25 << 20) + 4, n)):  # (16-byte aligned, odd end)
+        ops.adam(b[0][lo:hi], grad[lo:hi], b[1][lo:hi], b[2][lo:hi], 1e-2, step, grad_scale=gs)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    p64, g64, m64, v64 = p.double(), grad.double() * gs, m.double(), v.double()
+    mw = m64 + (g64 - m64) * (1 - b1)
+    # three roundings of the difference's term, one of the sum
+    mtol = U * (4 * (g64 - m64).abs() * (1 - b1) + mw.abs())
+    close(a[1], mw, mtol, "m")
+    vw = b2 * v64 + (1 - b2) * g64 * g64
+    close(a[2], vw, 5 * U * vw, "v")
+    den = vw.sqrt() / (1 - b2 ** step) ** 0.5 + eps
+    upd = lr / (1 - b1 ** step) * mw / den
+    # the root of 5 u, its own, the corrections' (1 each), two divisions, a sum, two products: below 12 u
+    close(a[0], p64 - upd, 12 * U * upd.abs() + lr / (1 - b1 ** step) * mtol / den + U * (p64 - upd).abs() + 2 * U * upd.abs(),
+          "p")
+    clipped = [t.clone() for t in (p, m, v)]
+    norm = ops.adam(clipped[0], grad, clipped[1], clipped[2], 1e-2, step, grad_scale=gs, max_norm=float("inf"))
+    assert all(torch.equal(x, y) for x, y in zip(a, clipped))
+    want = norm64([grad]) * gs
+    assert abs(float(norm) - want) <= 2 * U * want
+
+
 def test_arena_step_is_clipped(dev):
     """AdamState.apply(max_norm=...): padded views and fused groups; the padding adds nothing to the norm."""
     torch.manual_seed(0)
@@ -926,6 +1020,57 @@ def test_chain(dev):
     assert abs(float(got_loss) - float(loss)) <= 1e-6 and abs(float(got_norm) - float(norm)) <= 1e-5 * float(norm)
     for g, r in zip(grads + [h.grad], [p.grad for p in ref] + [hr.grad]):
         assert (g.double().cpu() - r).norm() <= 1e-5 * r.norm()
+
+
+@pytest.mark.parametrize("form", ["policy", "preference"])
+def test_gradients_into_the_generator(dev, form):
+    """The losses behind the framework's own generator: gradients of its LSTM and projection, of the words and of the code
+    against the same model in 64-bit torch on the CPU."""
+    from ldrs_amd.model.generator import Generator
+    from ldrs_amd.utils.config import Config
+    torch.manual_seed(3)
+    cfg = Config(7, 5, 50, 20, 1e-3, 7.9, 0.1, 0.1, 1.0, word_embed_size=12, latent_variable_size=6, decoder_rnn_size=20)
+    B, T, V, E, Z = 6, 7, 50, 12, 7
+    net = Generator(cfg).to(dev)
+    words = torch.randn(B, T, E, device=dev, generator=gen(1)).requires_grad_()
+    code = torch.randn(B, Z, device=dev, generator=gen(2)).requires_grad_()
+    t = torch.randint(0, V, (B * T,), device=dev, generator=gen(3))
+    A = torch.randn(B * T, device=dev, generator=gen(4))
+    w = (torch.arange(T, device=dev)[None] < torch.tensor([[7], [5], [7], [1], [6], [3]], device=dev)).float()
+    shift = 0.05 * torch.randn(B * T, device=dev, generator=gen(5))
+    sref = -20 + torch.randn(B, device=dev, generator=gen(6))
+
+    rnn = torch.nn.LSTM(E + Z, 20, num_layers=2, batch_first=True).double()
+    rnn.load_state_dict({k: v.double().cpu() for k, v in net.rnn.state_dict().items()})
+    fc = torch.nn.Linear(20, V).double()
+    fc.load_state_dict({k: v.double().cpu() for k, v in net.fc.state_dict().items()})
+    w64, c64 = [u.detach().double().cpu().requires_grad_() for u in (words, code)]
+    z = fc(rnn(torch.cat((w64, c64[:, None].expand(B, T, Z)), 2))[0].reshape(B * T, 20))
+    lp = torch.log_softmax(z, 1).gather(1, t.cpu()[:, None])[:, 0]
+    old = (lp.detach() - shift.double().cpu()).float()
+    wd = w.double().cpu().view(-1)
+    if form == "policy":
+        rho, Ad = (lp - old.double()).exp(), A.double().cpu()
+        want = -(wd * torch.minimum(rho * Ad, rho.clamp(0.8, 1.2) * Ad)).sum()
+    else:
+        gain = (wd * lp).view(B, T).sum(1) - sref.double().cpu()
+        want = -torch.nn.functional.logsigmoid(0.1 * (gain[:B // 2] - gain[B // 2:])).mean()
+    want.backward()
+
+    logits, _ = net(words, code, 0.0)
+    logits = logits.view(B * T, V)
+    if form == "policy":
+        loss = hnn.policy_loss(logits, t, A, w.view(-1), old_logp=old.to(dev))[0]
+    else:
+        loss = hnn.preference_loss(logits, t, w, sref, beta=0.1)[0]
+    loss.backward()
+    # norms: 2 layers of 7 steps there and back, 8 u a step, and 64 u for the projection and the loss: below 300 u
+    assert abs(float(loss.detach()) - float(want.detach())) <= 300 * U * float((wd * lp.detach().abs()).sum())
+    pairs = list(zip(net.rnn.flat_weights(), [getattr(rnn, k + "_l%d" % l) for l in (0, 1) for k in
+                                              ("weight_ih", "weight_hh", "bias_ih", "bias_hh")]))
+    pairs += [(net.fc.weight, fc.weight), (net.fc.bias, fc.bias), (words, w64), (code, c64)]
+    for k, (a, b) in enumerate(pairs):
+        assert (a.grad.double().cpu() - b.grad).norm() <= 300 * U * b.grad.norm(), k
 
 
 def test_other_streams(dev):
