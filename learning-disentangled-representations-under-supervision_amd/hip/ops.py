@@ -1581,6 +1581,7 @@ def _token_rows(logits, target, weight, inv_tau, dyn):
     _req(logits.dim() == 2 and logits.shape[1] > 0 and (logits.stride(1) == 1 or logits.shape[1] == 1),
          "logits must be [M,V] with unit column stride")
     M, V = logits.shape
+    _req(M < 2 ** 31 and V < 2 ** 31, "logits must have fewer than 2^31 rows and columns")
     ld = logits.stride(0) if M > 1 else V
     _req(ld >= V, "rows of logits must not overlap")
     dev = logits.device

@@ -196,6 +196,17 @@ def test_token_loss_refusals(host):
     assert len(host) == 3
 
 
+def test_vocabularies_past_32_bits_are_refused(host):
+    """The library counts a row's columns in 32 bits: 2^32 + 5 of them would pass for 5."""
+    x = torch.empty(1, 2 ** 32 + 5, dtype=torch.bfloat16)  # (8.6 GB that nothing touches)
+    i, v = torch.zeros(1, dtype=torch.int64), torch.zeros(1)
+    for f in (lambda: ops.token_logp(x, i), lambda: ops.policy_loss(x, i, v),
+              lambda: ops.token_logp_bwd(x, i, torch.zeros(1, 2), v, dlogits=x)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            f()
+    assert not host
+
+
 def test_clip_refusals(host):
     x = torch.zeros(6, 4)
     bad = [
