@@ -658,7 +658,8 @@ int cgn_policy_loss(void* stream, const cgn_token_rows* rows, const float* advan
 /* Preference loss over P = M / (2 T) pairs of sentences of T rows each (sentences 0..P-1 chosen, P..2P-1 rejected):
  *   S_j = sum_t weight * lp,  m_p = beta * ((S_p - ref_p) - (S_{P+p} - ref_{P+p}))
  *   loss = mean_p (-(1 - label_smoothing) log sigmoid(m_p) - label_smoothing log sigmoid(-m_p))
- * beta > 0, 0 <= label_smoothing < 0.5; margin [P] = m, seq_logp [2P] = S; stats, coef, dlogits and workspace as above. */
+ * beta > 0, 0 <= label_smoothing < 0.5; margin [P] = m, seq_logp [2P] = S; stats, coef, dlogits and workspace as above.
+ * A rejected sentence with a token of probability zero has m = +inf and, without smoothing, loss and gradient 0. */
 int cgn_preference_loss(void* stream, const cgn_token_rows* rows, int32_t T, const float* ref_logp, double beta,
                         double label_smoothing, float* loss, float* margin, float* seq_logp, float* stats, float* coef,
                         void* dlogits, int64_t ldd, void* workspace, int64_t workspace_bytes);

@@ -2,9 +2,10 @@
 //   mu = mean(x), var = mean((x - mu)^2), r = 1 / sqrt(var + eps), xh = (x - mu) r, y = xh w + b
 //   g = dy w,  dx = r (g - mean(g) - xh mean(g xh)),  dw = sum over rows dy xh,  db = sum over rows dy
 // HBM-bound (8 to 22 flops per element): every row is read once into registers and stays there for all its sums. A group
-// of G lanes owns a row; each lane holds NV 16-byte pieces of it. 83968 x 1024 bf16: forward 62 us (5.6 TB/s), backward
-// 101 us (5.1 TB/s); fp32 rows of 300 to 4096 elements run at 4.7 to 5.6 TB/s, bf16 rows of odd width (every second one at
-// an odd address) at 4.2 to 4.8 forward and 3.4 to 3.8 backward.
+// of G lanes owns a row; each lane holds NV 16-byte pieces of it. 83968 x 1024 bf16: forward 65 us (5.3 TB/s), backward
+// 98 to 101 us (5.1 to 5.3 TB/s); fp32 rows of 300 to 4096 elements run at 4.7 to 5.6 TB/s, bf16 rows of odd width at 4.2 to
+// 4.8 forward and 3.4 to 3.8 backward: a row's pieces start at its first element, so a wave's accesses there begin inside a
+// 128-byte line (token_loss.hip cuts its rows at the lines).
 #include "rows.h"
 
 namespace {
@@ -329,10 +330,16 @@ int launch_fwd(hipStream_t s, const void* x, int64_t ldx, int64_t R, int C, cons
     return CGN_OK;
 }
 
-// Workgroups of a backward pass. WAVES: waves per CU that the variant's registers leave room for; as many workgroups walk
-// the rows, and leave a row of `part` each (more would only lengthen the reduction behind them). A few rows take one
-// workgroup and one launch, with no reduction: at 10 x 800 fp32 (three workgroups' rows) a call from Python takes 14 us
-// instead of 18, in a graph 6.7 instead of 6.4; at 32 x 800 (eight) it would be 12.4 instead of 6.5 in a graph.
+// Workgroups of a backward pass. WAVES: waves per CU that the grid is made for; as many workgroups walk the rows, and
+// leave a row of `part` each (more would only lengthen the reduction behind them). A variant of up to 128 registers has
+// room for 16 waves, up to 168 for 12. Those that do not go by it: fp32 rows of up to 256 elements (78 to 80 registers,
+// room for 24, get 16), of 513 to 1024 (157 registers, room for 12, get 8: as fast) and of 1025 to 2048 (112, room for
+// 16, get 12), bf16 rows of 1025 to 2048 (103, room for 16, get 12); and fp32 rows of 2049 to 4096, whose 130 registers
+// leave room for one workgroup of 8 waves where the grid is made for two, which makes two rounds of it. From LN_ALONE
+// workgroups' rows on a group starts with one row only: at 1280 x 825 fp32 `part` then is half the size of x, and the
+// two launches take 7.3 and 4.2 us. A few rows take one workgroup and one launch, with no reduction: at 10 x 800 fp32
+// (three workgroups' rows) a call from Python takes 14 us instead of 18, in a graph 6.7 instead of 6.4; at 32 x 800
+// (eight) it would be 12.4 instead of 6.5 in a graph.
 template <int NT, int G, int WAVES>
 int64_t bwd_blocks(int64_t R) {
     const int64_t per = NT / G, nb = (R + per - 1) / per, most = 256 * WAVES * 64 / NT;
@@ -392,8 +399,8 @@ int norm_fwd(hipStream_t s, const void* x, int64_t ldx, int64_t R, int C, const 
 #undef LN_FWD
 }
 
-// A lane's share of a row is kept at 16 elements: row, gradient, weight, the two sums and the next row's loads fit 128 to
-// 160 registers.
+// A lane's share of a row is 4 to 16 elements: with gradient, weight, the two sums and the next row's loads 78 to 157
+// registers. The widest fp32 rows (4097 to 8192 elements, 1024 threads) are held to 128 and spill 12 bytes a lane.
 template <typename T>
 int norm_bwd(hipStream_t s, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t R, int C, const float* w,
              const float* mean, const float* rstd, void* dx, int64_t lddx, float* dw, float* db, float beta, float* part,

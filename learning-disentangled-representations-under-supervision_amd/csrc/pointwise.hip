@@ -301,7 +301,7 @@ __device__ __forceinline__ void adam_store(float* p, long i, f32x4 x) {
 // instead of 4 of 4 bytes); element by element the arithmetic is adam_kernel's, so the results are bit-identical. The
 // generator's arena (14.3 M parameters, 400 MB of traffic) is the step's largest HBM-bound kernel.
 // STREAM: arenas of 128 MB and more pass the caches by (non-temporal accesses; the same arithmetic, the same bits), in
-// 65536 workgroups of few trips: 64 M parameters (1.8 GB) in 268 us, 6.7 TB/s. With 8192 workgroups 301 us, without the
+// 65536 workgroups of few trips: 64 M parameters (1.8 GB) in 260 to 264 us, 6.8 TB/s. With 8192 workgroups 301, without the
 // non-temporal marks 335 us, and the next reader of the gradients waits for dirty lines besides (norm pass 44 -> 85 us).
 template <bool STREAM>
 __global__ __launch_bounds__(PW_NT) void adam_vec4_kernel(float* __restrict__ p, const float* __restrict__ g,

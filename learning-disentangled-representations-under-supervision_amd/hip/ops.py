@@ -1641,8 +1641,9 @@ def policy_loss(logits, target, advantage, weight=None, *, old_logp=None, ref_lo
       loss = sum_i weight_i (-min(rho A, clip(rho, 1 - clip[0], 1 + clip[1]) A) + kl_coef (exp(k) - k - 1)),
       k = ref_logp - logp
     logits [M,V] float32 or bfloat16; target int64 [M]; advantage, weight (None: ones), old_logp, ref_logp float32 [M].
-    Rows of weight zero are not read and contribute nothing. For the mean over the tokens that count, divide the weights
-    by their sum. dlogits: destination of d loss / d logits (the logits' own buffer is allowed).
+    Rows of weight zero are not read and contribute nothing. A row without a log-probability (target outside the
+    vocabulary, NaN logit) makes the loss and its own gradient NaN. For the mean over the tokens that count, divide the
+    weights by their sum. dlogits: destination of d loss / d logits (the logits' own buffer is allowed).
     save: also return (stats, coef) for token_logp_bwd."""
     r, M, V, ld, dev = _token_rows(logits, target, weight, inv_tau, dyn)
     _vector(advantage, M, "advantage", dev)
@@ -1669,7 +1670,9 @@ def preference_loss(logits, target, weight, ref_logp, *, beta, label_smoothing=0
       loss = mean_p -(1 - label_smoothing) log sigmoid(margin_p) - label_smoothing log sigmoid(-margin_p)
     weight: float32 [2P, T]; sentences 0..P-1 are the preferred ones, P..2P-1 the others of the same pairs; logits
     [2P*T, V] and target [2P*T] hold their rows sentence by sentence; tokens of weight zero (padding) are not read.
-    ref_logp: float32 [2P], the sentences' log-probabilities under the reference model. dlogits, save: as policy_loss."""
+    ref_logp: float32 [2P], the sentences' log-probabilities under the reference model. A sentence with a token of
+    probability zero has S = -inf: rejected, its pair's loss and gradient are 0 without smoothing. dlogits, save: as
+    policy_loss."""
     r, M, V, ld, dev = _token_rows(logits, target, weight, inv_tau, dyn)
     _req(weight is not None and weight.dim() == 2 and weight.shape[0] % 2 == 0 and M > 0,
          "weight must be [2P,T] with P, T >= 1")
