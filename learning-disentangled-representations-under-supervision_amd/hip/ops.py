@@ -1471,10 +1471,10 @@ def _own_or_apart(dst, ldd, src, lds, rows, cols, name):
              "%s must be the source's own buffer or lie apart from it" % name)
 
 
-def _overlap(t, n, u, m):
-    """Whether the first n elements from t's start on share memory with the first m from u's."""
-    a, b = t.data_ptr(), u.data_ptr()
-    return n > 0 and m > 0 and a < b + m * u.element_size() and b < a + n * t.element_size()
+def _range(t, n):
+    """First byte and end of n elements from t's start on."""
+    a = t.data_ptr()
+    return a, a + n * t.element_size()
 
 
 def _vector(t, n, name, dev):
@@ -1554,12 +1554,17 @@ def layer_norm_bwd(dy, x, weight, mean, rstd, dx=None, dweight=None, dbias=None,
                 _vector(dbias, Cn, "dbias", dev)
             else:
                 dbias = alloc((Cn,), dev)
-            spans = [(x, ldx, Cn, R), (dy, lddy, Cn, R), (dx, lddx, Cn, R), (weight, Cn, Cn, 1), (mean, R, R, 1),
-                     (rstd, R, R, 1)]
-            spans = [(t, (rows - 1) * ld + n if rows else 0) for t, ld, n, rows in spans if t is not None]
-            _req(not any([_overlap(d, Cn, t, n) for d in given for t, n in spans])
-                 and not (len(given) == 2 and _overlap(dweight, Cn, dbias, Cn)),
-                 "dweight and dbias must not overlap each other, an operand or dx")
+            if given:
+                taken = [_range(t, (R - 1) * ld + Cn if R else 0) for t, ld in ((x, ldx), (dy, lddy), (dx, lddx))
+                         if t is not None] + [_range(mean, R), _range(rstd, R)]
+                if weight is not None:
+                    taken.append(_range(weight, Cn))
+                for t in given:
+                    lo, hi = _range(t, Cn)
+                    for a, b in taken:
+                        if a < hi and lo < b and a < b:
+                            raise ValueError("dweight and dbias must not overlap each other, an operand or dx")
+                    taken.append((lo, hi))
         nb = C.c_int64()
         _lib.check(_lib.load().cgn_layer_norm_bwd_workspace(R, Cn, b16, C.byref(nb)), "cgn_layer_norm_bwd_workspace")
         if nb.value:
